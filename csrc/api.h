@@ -491,4 +491,59 @@ void attn_decode_split(const AttnCacheArgs& a, cudaStream_t s);
 void silu_mul_f16(const void* gate, const void* up, void* out, long long rows, int cols, long long g_ld,
                   long long u_ld, long long o_ld, cudaStream_t s);
 
+// ------------------------------------------------------------- llm/paged_append.cu, paged_attention.cu
+// A paged key / value cache: k and v are [n_pages][Hkv][page][D] (same strides, D contiguous); position p of sequence s
+// lives in row p % page of page table[s][p / page].  Table entries, sequence numbers, positions and lengths come from
+// device data: a bad one is recorded as RT_ERR_BOUNDS and its access skipped.  Sequence number -1 marks a padded token.
+struct PagedCache {
+  void *k, *v;
+  long long s_page, s_head, s_row;  // strides in elements
+  int n_pages, Hkv, page, D;
+  const int* table;  // [n_seq][max_pages], row stride table_stride
+  long long table_stride;
+  int n_seq, max_pages;
+};
+struct PagedAppendArgs {
+  int dtype;  // DT_F16 or DT_BF16
+  PagedCache cache;
+  const void *q, *k, *v;  // [n_tok][H][D], [n_tok][Hkv][D], strides in elements, D contiguous
+  long long q_st, q_sh, k_st, k_sh, v_st, v_sh;
+  void *q_out, *k_out;    // rotated q and (or null) rotated k
+  long long qo_st, qo_sh, ko_st, ko_sh;
+  const int *pos, *seq;   // [n_tok]; seq null: token t belongs to sequence t
+  const float* inv_freq;  // [rot / 2]
+  const void *q_norm, *k_norm;  // [D] RMSNorm weights or null
+  float eps;
+  int n_tok, H, rot, interleaved;
+};
+void paged_append(const PagedAppendArgs& a, cudaStream_t s);
+struct PagedAttnArgs {
+  int dtype;
+  PagedCache cache;
+  const void* q;  // [n_tok][H][D]
+  long long q_st, q_sh;
+  void* out;
+  long long o_st, o_sh;
+  const int *kv_len, *seq;  // [n_tok]; token t sees positions [max(0, kv_len - window), kv_len) of its sequence
+  int n_tok, H, window;     // window 0: no limit
+  float scale, softcap;     // softcap 0: none
+};
+void paged_attention(const PagedAttnArgs& a, cudaStream_t s);
+// ------------------------------------------------------------- llm/sample_tokens.cu
+struct SampleArgs {
+  int dtype;           // DT_F32, DT_F16 or DT_BF16
+  const void* logits;  // [rows][vocab], row stride ld
+  long long ld;
+  int rows, vocab;
+  const void* uniform;  // [rows] fp32 or fp64 (uniform_f64)
+  bool uniform_f64;
+  // one value per row, or null: the scalar for every row
+  const float *temperature_rows, *top_p_rows, *min_p_rows;
+  const int* top_k_rows;
+  double temperature, top_p, min_p;
+  int top_k;
+  long long* out;  // [rows]
+};
+void sample_tokens(const SampleArgs& a, cudaStream_t s);
+
 }  // namespace rt

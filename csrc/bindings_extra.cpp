@@ -1018,7 +1018,10 @@ void im2col_nhwc(const Tensor& x, Tensor& col, int64_t KH, int64_t KW, int64_t s
                   int(col.size(1)), cur_stream(x.device().index()));
 }
 
+void register_serving_ops(pybind11::module_& m);  // bindings_serving.cpp
+
 void register_extra_ops(pybind11::module_& m) {
+  register_serving_ops(m);
   m.def("im2col_nhwc", &im2col_nhwc, "patch matrix of a channels-last bf16 image (few input channels)");
   m.def("p2p_collective", &p2p_collective, "all-reduce / all-gather / reduce-scatter / broadcast over symmetric peer memory");
   m.def("rope_split", &rope_split, "rotary embedding fused with the q / k / v split (bf16), forward or backward");
