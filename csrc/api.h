@@ -528,7 +528,15 @@ struct PagedAttnArgs {
   int n_tok, H, window;     // window 0: no limit
   float scale, softcap;     // softcap 0: none
 };
-void paged_attention(const PagedAttnArgs& a, cudaStream_t s);
+constexpr int PAGED_ATTN_CHUNK = 512;           // tokens of one launch
+constexpr int PAGED_ATTN_COUNTER_BYTES = 8192;  // at the start of the workspace: zeros before its first use, left zero by every call
+struct PagedAttnPlan {
+  int grid;
+  long long workspace_bytes;  // for any call of this head size on this device
+};
+PagedAttnPlan paged_attention_plan(const PagedAttnArgs& a);
+// `workspace` may serve one launch at a time: calls that can run at once need one each
+void paged_attention(const PagedAttnArgs& a, const PagedAttnPlan& p, void* workspace, cudaStream_t s);
 // ------------------------------------------------------------- llm/sample_tokens.cu
 struct SampleArgs {
   int dtype;           // DT_F32, DT_F16 or DT_BF16

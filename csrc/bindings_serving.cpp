@@ -1,9 +1,13 @@
 // Bindings of the token-serving operators: paged cache append, paged attention, token sampling.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
+#include <map>
+#include <mutex>
 
 #include "api.h"
 #include "common/launch.h"
@@ -123,6 +127,25 @@ Tensor paged_append(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
   return out;
 }
 
+// Parts of items that several CTAs share, behind zeroed arrival counters.  Calls on one stream follow one another, so a stream keeps
+// one buffer; a captured graph may replay beside anything else, so each captured call gets memory of the graph's own.
+Tensor attention_workspace(const Tensor& like, int64_t bytes) {
+  const auto opts = like.options().dtype(at::kByte);
+  const cudaStream_t stream = stream_of(like);
+  auto fresh = [&]() {
+    Tensor t = at::empty({bytes}, opts);
+    C10_CUDA_CHECK(cudaMemsetAsync(t.data_ptr(), 0, rt::PAGED_ATTN_COUNTER_BYTES, stream));
+    return t;
+  };
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return fresh();
+  static std::mutex mu;
+  static auto* kept = new std::map<std::pair<int, cudaStream_t>, Tensor>();  // outlives the allocator's own shutdown
+  std::lock_guard<std::mutex> lock(mu);
+  Tensor& t = (*kept)[{like.device().index(), stream}];
+  if (!t.defined() || t.numel() < bytes) t = fresh();
+  return t;
+}
+
 Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& kv_len,
                        const OptTensor& seq, double scale, int64_t window, double softcap, const OptTensor& out_) {
   const char* op = "paged_attention";
@@ -159,7 +182,10 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& 
   a.window = int(std::min<int64_t>(window, INT32_MAX));
   a.scale = float(scale);
   a.softcap = float(softcap);
-  rt::paged_attention(a, stream_of(q));
+  if (n == 0) return out;
+  const rt::PagedAttnPlan plan = rt::paged_attention_plan(a);
+  const Tensor workspace = attention_workspace(q, plan.workspace_bytes);
+  rt::paged_attention(a, plan, workspace.data_ptr(), stream_of(q));
   return out;
 }
 
