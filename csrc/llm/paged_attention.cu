@@ -6,15 +6,17 @@
 // A token that sees no position gets zeros.  Every visible key and value is read once per (token, kv head): the cache's
 // bytes are the bound (4 D bytes for 4 D H / Hkv operations), so the kernel is built around keeping loads in flight.
 //
-// Work: a (token, kv head, 16 of its query heads) is an item, its visible positions are cut into units of 64 keys.  The
-// units of all items, in order, are dealt to a fixed grid in equal contiguous shares, from the lengths on the device:
-// ragged batches stay balanced, one long sequence uses the whole GPU, and a captured launch fits every later length.  An item
-// that lies in one share is finished there; one that was cut leaves (max, sum, output) parts, and whichever CTA arrives
-// last at its counter joins them in share order, so the result does not depend on timing.
+// Work: a (token, kv head, up to 8 or 16 of its query heads) is an item, its visible positions are cut into units of 64
+// keys.  The units of all items, in order, are dealt to a fixed grid in equal contiguous shares, from the lengths on the
+// device: ragged batches stay balanced, one long sequence uses the whole GPU, and a captured launch fits every later length.  An
+// item that lies in one share is finished there; one that was cut leaves (max, sum, output) parts, and whichever CTA
+// arrives last at its counter joins them in share order, so the result does not depend on timing.
 //
 // Inside a CTA each of four warps owns 16 keys of a unit and its own ring of cp.async stages, without block barriers
-// between units; the ring runs on across items.  Scores and outputs are m16n8k16 products with the item's query heads as
-// the 16 rows (decode has too few rows for the 128-row tcgen05 tiles, and the tensor time here is a fraction of the load time).
+// between units; the ring runs on across items.  The products are m16n8k16 with the cache as the 16 rows and eight query
+// heads as the columns: S^T = K Q^T (16 keys), O^T += V^T P^T (16 of D).  Decode has 1 to 16 query heads a kv head, a
+// corner of a 128-row tcgen05 tile; here the tensor time is a fraction of the load time.  A lane copies parts of exactly
+// the two key rows whose scores it later holds, so its page look-ups give its mask too.
 // Maximum, sum and output are kept in 32 bits.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -32,22 +34,27 @@ namespace rt {
 namespace {
 
 constexpr int PA_WARPS = 4;
-constexpr int PA_TILE = 16;                    // keys of one warp step, and query heads of an item
+constexpr int PA_TILE = 16;                    // keys of one warp step
 constexpr int PA_UNIT = PA_WARPS * PA_TILE;    // keys of one CTA step
 constexpr float PA_LOG2E = 1.4426950408889634f;
+// The running maximum is moved only when a score exceeds it by PA_SLACK (base 2), and then set PA_ROOM below the score: weights
+// reach 2^14 at most, which fits fp16, and small ones keep more of its digits than with the maximum itself.
+constexpr float PA_SLACK = 14.f, PA_ROOM = 4.f;
 
-template <typename T, int DP> struct Cfg {
+template <int DP, int NH> struct Cfg {         // DP: head size rounded up, NH: eights of query heads in an item
+  static constexpr int HEADS = 8 * NH;
   static constexpr int ROW = DP * 2 + 16;                      // bytes of a staged row: 16 more than the data keep ldmatrix conflict-free
   static constexpr int STAGES = DP <= 96 ? 3 : 2;
   static constexpr int STAGE = 2 * PA_TILE * ROW;              // one warp's K and V rows
-  static constexpr int QBUF = PA_TILE * ROW;
-  static constexpr int ACC_LD = DP + 8;                        // floats of a row of the merge buffer
+  static constexpr int QBUF = HEADS * ROW;
+  static constexpr int ACC_LD = DP + 4;                        // floats of a row of the merge buffer
   static constexpr int OFF_Q = STAGES * PA_WARPS * STAGE;
   static constexpr int OFF_ACC = OFF_Q + (STAGES + 1) * QBUF;
-  static constexpr int OFF_ML = OFF_ACC + 2 * PA_TILE * ACC_LD * 4;
-  static constexpr int OFF_TOK = OFF_ML + 2 * PA_WARPS * PA_TILE * 4;
+  static constexpr int OFF_ML = OFF_ACC + 2 * HEADS * ACC_LD * 4;
+  static constexpr int OFF_TOK = OFF_ML + 2 * PA_WARPS * HEADS * 4;
   static constexpr int SMEM = OFF_TOK + PAGED_ATTN_CHUNK * 20 + 8;
-  static constexpr bool Q_IN_REGS = DP <= 128;
+  static constexpr int PART = HEADS * (DP + 2);                // floats of a part: rows, maxima, sums
+  static constexpr bool Q_IN_REGS = DP * NH <= 256;
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool full) {  // zero-fills where not full
@@ -60,6 +67,11 @@ __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
 }
 __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {  // of 16-bit values across the warp
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -84,22 +96,22 @@ __device__ __forceinline__ int units_of(int lo, int len) { return (int)(((unsign
 
 // A walk over the units of this CTA's share.
 struct Walk {
-  int t, hr;       // token; kv head * row tiles + row tile
+  int t, hr;       // token; kv head * head groups + head group
   int v, nu;       // unit within the item, units of the item
 };
 
-template <typename T, int DP>
+template <typename T, int DP, int NH>
 __global__ void __launch_bounds__(PA_WARPS * 32)
-paged_attention_kernel(PagedAttnArgs a, int t0, int n, float* __restrict__ part, int* __restrict__ counters, int* __restrict__ status) {
-  using C = Cfg<T, DP>;
-  constexpr int S = C::STAGES, CH = DP / 8, NT = DP / 8, KS = DP / 16;
+paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, int t0, int n, float* __restrict__ part,
+                       int* __restrict__ counters, int* __restrict__ status) {
+  using C = Cfg<DP, NH>;
+  constexpr int S = C::STAGES, CH = DP / 8, CL = CH / 4, KS = DP / 16, NT = DP / 16, HEADS = C::HEADS;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ long long sm_scan[PA_WARPS];
-  __shared__ int sm_mask[PA_WARPS][S];
   __shared__ int sm_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const PagedCache& c = a.cache;
-  const int G = a.H / c.Hkv, RT = (G + PA_TILE - 1) / PA_TILE, HR = c.Hkv * RT;
+  const int G = a.H / c.Hkv, RT = (G + HEADS - 1) / HEADS, HR = c.Hkv * RT;
   const int chunks = c.D >> 3;
   Tokens tk;
   tk.first = reinterpret_cast<long long*>(smem + C::OFF_TOK);
@@ -191,68 +203,88 @@ paged_attention_kernel(PagedAttnArgs a, int t0, int n, float* __restrict__ part,
   }
   Walk cw = ld;
 
-  // ---- loads: lane r < 16 looks up the page of the tile's key r one tile ahead
+  // ---- loads: lane copies 16-byte chunks lane % 4, + 4, .. of key rows lane / 4 and lane / 4 + 8; pages are looked up one tile ahead
   const uint32_t sbase = smem_u32(smem);
-  const uint32_t my_stage = sbase + warp * C::STAGE;
-  long long lu = ub;
+  const uint32_t my_stage = sbase + warp * C::STAGE + (lane >> 2) * C::ROW + (lane & 3) * 16;
+  const T* const nothing = (const T*)a.q;  // source address of copies that only write zeros
+  const int ch0 = lane & 3;
+  const T* const kbase = (const T*)c.k + ch0 * 8;
+  const T* const vbase = (const T*)c.v + ch0 * 8;
+  long long left = ue - ub;                // units to load
   int ld_items = 0;
   bool ld_new = true;
-  int pg = -1, row_in_page = 0;
+  unsigned j0, jn;                         // this lane's first key of the next tile, the sequence's end
+  const int* pages;
+  long long head_off;
+  auto enter_item = [&]() {
+    jn = (unsigned)tk.len[ld.t];
+    j0 = (unsigned)tk.lo[ld.t] + (unsigned)ld.v * PA_UNIT + warp * PA_TILE + (lane >> 2);
+    pages = c.table + tk.seq[ld.t] * c.table_stride;
+    head_off = (long long)(ld.hr / RT) * c.s_head;
+  };
+  int pg[2], row[2];
   auto look_up = [&]() {
-    pg = -1;
-    if (lu < ue && lane < PA_TILE) {
-      const unsigned j = (unsigned)tk.lo[ld.t] + (unsigned)ld.v * PA_UNIT + warp * PA_TILE + lane;
-      if (j < (unsigned)tk.len[ld.t]) {
-        const unsigned k = j / (unsigned)c.page;
-        row_in_page = (int)(j - k * c.page);
-        pg = __ldcg(c.table + tk.seq[ld.t] * c.table_stride + k);
-        if (pg < 0 || pg >= c.n_pages) {
-          pg = -1;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const unsigned j = j0 + 8 * e;
+      pg[e] = -1;
+      if (j < jn) {
+        const unsigned k = __umulhi(2 * j, page_mul) >> page_shift;  // j / page
+        row[e] = (int)(j - k * c.page);
+        pg[e] = __ldcg(pages + k);
+        if (pg[e] < 0 || pg[e] >= c.n_pages) {
+          pg[e] = -1;
           atomicCAS(status, 0, RT_ERR_BOUNDS);
         }
       }
     }
   };
+  unsigned seen = 0;  // two bits a stage: whether this lane's two keys count
   auto issue = [&](int stage) {
-    if (lu < ue) {
-      const unsigned mask = __ballot_sync(0xffffffffu, pg >= 0);
-      if (lane == 0) sm_mask[warp][stage] = (int)mask;
-      const int hk = ld.hr / RT;
-      if (ld_new) {  // this warp's four rows of the item's queries
-        const int r0 = (ld.hr - hk * RT) * PA_TILE;
+    if (left > 0) {
+      if (ld_new) {  // this warp's quarter of the item's query rows
+        const int hk = ld.hr / RT, r0 = (ld.hr - hk * RT) * HEADS;
         const uint32_t qd = sbase + C::OFF_Q + (ld_items % (S + 1)) * C::QBUF;
 #pragma unroll
-        for (int i = lane; i < 4 * CH; i += 32) {
-          const int r = warp * 4 + i / CH, ch = i % CH;
+        for (int i = lane; i < HEADS / 4 * CH; i += 32) {
+          const int r = warp * (HEADS / 4) + i / CH, ch = i % CH;
           const bool ok = r0 + r < G;
           if (ch < chunks)
             cp_async16(qd + r * C::ROW + ch * 16, (const T*)a.q + (ok ? (t0 + ld.t) * a.q_st + (long long)(hk * G + r0 + r) * a.q_sh : 0) + ch * 8, ok);
         }
         ++ld_items;
       }
-      if (mask) {
-        const long long off = (long long)(pg < 0 ? 0 : pg) * c.s_page + (long long)row_in_page * c.s_row + (long long)hk * c.s_head;
+      const bool ok[2] = {pg[0] >= 0, pg[1] >= 0};
+      seen = (seen & ~(3u << (2 * stage))) | ((ok[0] ? 1u : 0u) | (ok[1] ? 2u : 0u)) << (2 * stage);
+      if (__any_sync(0xffffffffu, ok[0] || ok[1])) {
         const uint32_t dst = my_stage + stage * (PA_WARPS * C::STAGE);
 #pragma unroll
-        for (int i = 0; i < PA_TILE * CH / 32; ++i) {
-          const int r = (i * 32 + lane) / CH, ch = (i * 32 + lane) % CH;
-          const long long o = __shfl_sync(0xffffffffu, off, r);
-          const bool ok = mask >> r & 1;
-          if (ch < chunks) {
-            cp_async16(dst + r * C::ROW + ch * 16, ok ? (const T*)c.k + o + ch * 8 : (const T*)a.q, ok);
-            cp_async16(dst + PA_TILE * C::ROW + r * C::ROW + ch * 16, ok ? (const T*)c.v + o + ch * 8 : (const T*)a.q, ok);
-          }
+        for (int e = 0; e < 2; ++e) {
+          const long long off = pg[e] * c.s_page + row[e] * c.s_row + head_off;
+          const T* const ks = ok[e] ? kbase + off : nothing;
+          const T* const vs = ok[e] ? vbase + off : nothing;
+#pragma unroll
+          for (int i = 0; i < CL; ++i)
+            if (ch0 + 4 * i < chunks) {
+              cp_async16(dst + e * 8 * C::ROW + i * 64, ok[e] ? ks + i * 32 : nothing, ok[e]);
+              cp_async16(dst + (PA_TILE + e * 8) * C::ROW + i * 64, ok[e] ? vs + i * 32 : nothing, ok[e]);
+            }
         }
       }
-      const int t_was = ld.t, h_was = ld.hr;
-      ++lu;
+      --left;
+      ld_new = ld.v + 1 == ld.nu;
+      j0 += PA_UNIT;
       step(ld);
-      ld_new = ld.t != t_was || ld.hr != h_was;
-      look_up();
+      pg[0] = pg[1] = -1;
+      if (left > 0) {
+        if (ld_new) enter_item();
+        look_up();
+      }
     }
     cp_commit();
   };
   __syncthreads();  // the zeroed columns are in place
+  enter_item();
   look_up();
 #pragma unroll
   for (int i = 0; i < S; ++i) issue(i);
@@ -262,98 +294,111 @@ paged_attention_kernel(PagedAttnArgs a, int t0, int n, float* __restrict__ part,
   const float cap2 = a.softcap * PA_LOG2E;
   float* acc_buf = reinterpret_cast<float*>(smem + C::OFF_ACC);
   float* sm_m = reinterpret_cast<float*>(smem + C::OFF_ML);
-  float* sm_l = sm_m + PA_WARPS * PA_TILE;
-  const uint32_t k_lane = ((lane >> 4) * 8 + (lane & 7)) * C::ROW + ((lane >> 3) & 1) * 16;
-  const uint32_t v_lane = (((lane >> 3) & 1) * 8 + (lane & 7)) * C::ROW + (lane >> 4) * 16;
+  float* sm_l = sm_m + PA_WARPS * HEADS;
+  // ldmatrix lanes: A fragments of K (rows are keys) and, transposed, of V; B fragments of Q
+  const uint32_t k_lane = sbase + warp * C::STAGE + ((lane & 7) + ((lane >> 3) & 1) * 8) * C::ROW + (lane >> 4) * 16;
+  const uint32_t v_lane = sbase + warp * C::STAGE + (PA_TILE + (lane & 7) + (lane >> 4) * 8) * C::ROW + ((lane >> 3) & 1) * 16;
   int stage = 0, item = 0;
   long long u = ub;
   while (u < ue) {
-    const int t = cw.t, hk = cw.hr / RT, r0 = (cw.hr - hk * RT) * PA_TILE, rows = min(PA_TILE, G - r0);
+    const int t = cw.t, hk = cw.hr / RT, r0 = (cw.hr - hk * RT) * HEADS, rows = min(HEADS, G - r0);
     const long long g0 = tk.first[t] + (long long)cw.hr * cw.nu, g1 = g0 + cw.nu;
     const long long end = min(g1, ue);
-    uint32_t qf[C::Q_IN_REGS ? KS : 1][4];
-    float o[NT][4], m0 = -CUDART_INF_F, m1 = -CUDART_INF_F, l0 = 0.f, l1 = 0.f;
+    uint32_t qf[C::Q_IN_REGS ? NH : 1][C::Q_IN_REGS ? KS / 2 : 1][4];
+    // this lane: heads 2 (lane % 4) + {0, 1} of each eight; rows (keys, or places in D) lane / 4 and lane / 4 + 8
+    float o[NH][NT][4], m[NH][2], l[NH][2];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    for (int h = 0; h < NH; ++h) {
+      m[h][0] = m[h][1] = -CUDART_INF_F;
+      l[h][0] = l[h][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) o[h][i][0] = o[h][i][1] = o[h][i][2] = o[h][i][3] = 0.f;
+    }
     cp_wait<S - 1>();
     __syncthreads();  // all four warps' query rows have arrived; the merge buffer is free again
-    // ldmatrix A fragments: rows 0-7 / 8-15, columns 0-7 / 8-15 of each 16 x 16 block
-    const uint32_t q_lane = sbase + C::OFF_Q + (item % (S + 1)) * C::QBUF + ((lane & 7) + ((lane >> 3) & 1) * 8) * C::ROW + (lane >> 4) * 16;
+    const uint32_t q_lane = sbase + C::OFF_Q + (item % (S + 1)) * C::QBUF + (lane & 7) * C::ROW + (lane >> 3) * 16;
     if constexpr (C::Q_IN_REGS) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) ldsm4(q_lane + ks * 32, qf[ks]);
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int k2 = 0; k2 < KS / 2; ++k2) ldsm4(q_lane + h * 8 * C::ROW + k2 * 64, qf[h][k2]);
     }
     for (; u < end; ++u) {
       cp_wait<S - 1>();
       __syncwarp();
-      const unsigned mask = (unsigned)sm_mask[warp][stage];
-      if (mask) {
-        const uint32_t ks_base = my_stage + stage * (PA_WARPS * C::STAGE);
-        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+      const bool ok0 = seen >> (2 * stage) & 1, ok1 = seen >> (2 * stage) & 2;
+      if (__any_sync(0xffffffffu, ok0 || ok1)) {
+        const uint32_t st = stage * (PA_WARPS * C::STAGE);
+        float s[NH][2][4];  // even and odd steps of D, so that two chains of products run at once
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          uint32_t b[4];
-          ldsm4(ks_base + k_lane + ks * 32, b);
-          if constexpr (C::Q_IN_REGS) {
-            mma16816<T>(s0, qf[ks], b[0], b[1]);
-            mma16816<T>(s1, qf[ks], b[2], b[3]);
-          } else {
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[h][0][e] = s[h][1][e] = 0.f;
+#pragma unroll
+        for (int k2 = 0; k2 < KS / 2; ++k2) {
+          uint32_t ka[4], kb[4];
+          ldsm4(k_lane + st + k2 * 64, ka);
+          ldsm4(k_lane + st + k2 * 64 + 32, kb);
+#pragma unroll
+          for (int h = 0; h < NH; ++h) {
             uint32_t q4[4];
-            ldsm4(q_lane + ks * 32, q4);
-            mma16816<T>(s0, q4, b[0], b[1]);
-            mma16816<T>(s1, q4, b[2], b[3]);
+            if constexpr (C::Q_IN_REGS) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) q4[e] = qf[h][k2][e];
+            } else {
+              ldsm4(q_lane + h * 8 * C::ROW + k2 * 64, q4);
+            }
+            mma16816<T>(s[h][0], ka, q4[0], q4[1]);
+            mma16816<T>(s[h][1], kb, q4[2], q4[3]);
           }
         }
-        // thread: rows lane / 4 (elements 0, 1) and lane / 4 + 8 (2, 3); keys 2 (lane % 4) + {0, 1}, and 8 more in s1
-        const unsigned mk = mask >> (2 * (lane & 3));
+        bool grow = false;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s0[e] *= scale2;
-          s1[e] *= scale2;
-          if (a.softcap > 0.f) {  // tanh(x) = 1 - 2 / (exp(2x) + 1): its error is absolute, which is what a score's exponential sees
-            s0[e] = cap2 - 2.f * cap2 / (ex2_approx(s0[e]) + 1.f);
-            s1[e] = cap2 - 2.f * cap2 / (ex2_approx(s1[e]) + 1.f);
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x = (s[h][0][e] + s[h][1][e]) * scale2;
+            if (a.softcap > 0.f) x = cap2 - 2.f * cap2 / (ex2_approx(x) + 1.f);  // tanh(y) = 1 - 2 / (exp(2y) + 1), error absolute as a score's may be
+            x = (e < 2 ? ok0 : ok1) ? x : -CUDART_INF_F;
+            grow |= x > m[h][e & 1] + PA_SLACK;
+            s[h][0][e] = x;
           }
-          if (!(mk >> (e & 1) & 1)) s0[e] = -CUDART_INF_F;
-          if (!(mk >> (8 + (e & 1)) & 1)) s1[e] = -CUDART_INF_F;
-        }
-        float x0 = fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s1[0], s1[1])), x1 = fmaxf(fmaxf(s0[2], s0[3]), fmaxf(s1[2], s1[3]));
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-        if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
-          const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-          const float f0 = n0 == -CUDART_INF_F ? 1.f : ex2_approx(m0 - n0), f1 = n1 == -CUDART_INF_F ? 1.f : ex2_approx(m1 - n1);
-          m0 = n0;
-          m1 = n1;
-          l0 *= f0;
-          l1 *= f1;
+        if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            o[i][0] *= f0;
-            o[i][1] *= f0;
-            o[i][2] *= f1;
-            o[i][3] *= f1;
-          }
-        }
-        const float b0 = m0 == -CUDART_INF_F ? 0.f : m0, b1 = m1 == -CUDART_INF_F ? 0.f : m1;
+          for (int h = 0; h < NH; ++h)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          s0[e] = ex2_approx(s0[e] - b0);
-          s1[e] = ex2_approx(s1[e] - b0);
-          s0[2 + e] = ex2_approx(s0[2 + e] - b1);
-          s1[2 + e] = ex2_approx(s1[2 + e] - b1);
-        }
-        l0 += (s0[0] + s0[1]) + (s1[0] + s1[1]);
-        l1 += (s0[2] + s0[3]) + (s1[2] + s1[3]);
-        const uint32_t p[4] = {pack2<T>(s0[0], s0[1]), pack2<T>(s0[2], s0[3]), pack2<T>(s1[0], s1[1]), pack2<T>(s1[2], s1[3])};
+            for (int e = 0; e < 2; ++e) {
+              float x = fmaxf(s[h][0][e], s[h][0][e + 2]);
 #pragma unroll
-        for (int i = 0; i < NT; i += 2) {
-          uint32_t b[4];
-          ldsm4_t(ks_base + PA_TILE * C::ROW + v_lane + i * 16, b);
-          mma16816<T>(o[i], p, b[0], b[1]);
-          mma16816<T>(o[i + 1], p, b[2], b[3]);
+              for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+              if (x > m[h][e] + PA_SLACK) {
+                const float f = ex2_approx(m[h][e] - (x - PA_ROOM));
+                m[h][e] = x - PA_ROOM;
+                l[h][e] *= f;
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                  o[h][i][e] *= f;
+                  o[h][i][e + 2] *= f;
+                }
+              }
+            }
+        }
+        uint32_t p[NH][2];
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[h][0][e] = ex2_approx(s[h][0][e] - (m[h][e & 1] == -CUDART_INF_F ? 0.f : m[h][e & 1]));
+          l[h][0] += s[h][0][0] + s[h][0][2];
+          l[h][1] += s[h][0][1] + s[h][0][3];
+          p[h][0] = transpose8x8(pack2<T>(s[h][0][0], s[h][0][1]));  // weights enter the product rounded to the values' type
+          p[h][1] = transpose8x8(pack2<T>(s[h][0][2], s[h][0][3]));
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          uint32_t va[4];
+          ldsm4_t(v_lane + st + i * 32, va);
+#pragma unroll
+          for (int h = 0; h < NH; ++h) mma16816<T>(o[h][i], va, p[h][0], p[h][1]);
         }
       }
       __syncwarp();  // the stage is free
@@ -364,63 +409,67 @@ paged_attention_kernel(PagedAttnArgs a, int t0, int n, float* __restrict__ part,
     ++item;
 
     // ---- the four warps' states become one: warps 2, 3 hand over to 0, 1, whose sums all threads then add
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    const int ra = lane >> 2, rb = ra + 8;
-    if ((lane & 3) == 0) {
-      sm_m[warp * PA_TILE + ra] = m0;
-      sm_m[warp * PA_TILE + rb] = m1;
-      sm_l[warp * PA_TILE + ra] = l0;
-      sm_l[warp * PA_TILE + rb] = l1;
-    }
-    float* const buf = acc_buf + (warp & 1) * PA_TILE * C::ACC_LD + (lane & 3) * 2;
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[h][e] += __shfl_xor_sync(0xffffffffu, l[h][e], d);
+        if (lane < 4) {
+          sm_m[warp * HEADS + h * 8 + lane * 2 + e] = m[h][e];
+          sm_l[warp * HEADS + h * 8 + lane * 2 + e] = l[h][e];
+        }
+      }
+    float* const buf = acc_buf + (warp & 1) * HEADS * C::ACC_LD + (lane & 3) * 2 * C::ACC_LD + (lane >> 2);
     if (warp >= 2) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        if (ra < rows) *reinterpret_cast<float2*>(buf + ra * C::ACC_LD + i * 8) = make_float2(o[i][0], o[i][1]);
-        if (rb < rows) *reinterpret_cast<float2*>(buf + rb * C::ACC_LD + i * 8) = make_float2(o[i][2], o[i][3]);
-      }
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) buf[(h * 8 + (e & 1)) * C::ACC_LD + i * 16 + (e >> 1) * 8] = o[h][i][e];
     }
     __syncthreads();
     auto top = [&](int r) {
       float x = sm_m[r];
 #pragma unroll
-      for (int w = 1; w < PA_WARPS; ++w) x = fmaxf(x, sm_m[w * PA_TILE + r]);
+      for (int w = 1; w < PA_WARPS; ++w) x = fmaxf(x, sm_m[w * HEADS + r]);
       return x;
     };
     auto factor = [](float m, float big) { return big == -CUDART_INF_F ? 0.f : ex2_approx(m - big); };
     if (warp < 2) {
-      const float ta = top(ra), tb = top(rb);
-      const float fa = factor(m0, ta), fb = factor(m1, tb);
-      const float ga = factor(sm_m[(warp + 2) * PA_TILE + ra], ta), gb = factor(sm_m[(warp + 2) * PA_TILE + rb], tb);
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        if (ra < rows) {
-          float2* p = reinterpret_cast<float2*>(buf + ra * C::ACC_LD + i * 8);
-          *p = make_float2(fmaf(p->x, ga, o[i][0] * fa), fmaf(p->y, ga, o[i][1] * fa));
+      for (int h = 0; h < NH; ++h) {
+        float f[2], g[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = h * 8 + (lane & 3) * 2 + e;
+          const float big = top(r);
+          f[e] = factor(m[h][e], big);
+          g[e] = factor(sm_m[(warp + 2) * HEADS + r], big);
         }
-        if (rb < rows) {
-          float2* p = reinterpret_cast<float2*>(buf + rb * C::ACC_LD + i * 8);
-          *p = make_float2(fmaf(p->x, gb, o[i][2] * fb), fmaf(p->y, gb, o[i][3] * fb));
-        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float* x = buf + (h * 8 + (e & 1)) * C::ACC_LD + i * 16 + (e >> 1) * 8;
+            *x = fmaf(*x, g[e & 1], o[h][i][e] * f[e & 1]);
+          }
       }
     }
     __syncthreads();
     auto total = [&](int r, float big) {
       float x = 0.f;
 #pragma unroll
-      for (int w = 0; w < PA_WARPS; ++w) x += sm_l[w * PA_TILE + r] * factor(sm_m[w * PA_TILE + r], big);
+      for (int w = 0; w < PA_WARPS; ++w) x += sm_l[w * HEADS + r] * factor(sm_m[w * HEADS + r], big);
       return x;
     };
     T* const out = (T*)a.out + (t0 + t) * a.o_st + (long long)(hk * G + r0) * a.o_sh;
     const bool whole = g0 >= ub && g1 <= ue;
-    constexpr int PART = PA_TILE * (DP + 2);  // floats of a part: rows, maxima, sums
-    float* const slot = part + ((long long)blockIdx.x * 2 + (g0 >= ub ? 1 : 0)) * PART;
+    float* const slot = part + ((long long)blockIdx.x * 2 + (g0 >= ub ? 1 : 0)) * C::PART;
     for (int i = tid; i < rows * DP; i += PA_WARPS * 32) {
       const int r = i / DP, d = i % DP;
-      const float x = acc_buf[r * C::ACC_LD + d] + acc_buf[(PA_TILE + r) * C::ACC_LD + d];
+      const float x = acc_buf[r * C::ACC_LD + d] + acc_buf[(HEADS + r) * C::ACC_LD + d];
       if (whole) {
         const float l = total(r, top(r));
         if (d < c.D) put(out + r * a.o_sh + d, l == 0.f ? 0.f : x / l);
@@ -428,8 +477,8 @@ paged_attention_kernel(PagedAttnArgs a, int t0, int n, float* __restrict__ part,
         __stcg(slot + r * DP + d, x);
         if (d == 0) {
           const float big = top(r);
-          __stcg(slot + PA_TILE * DP + r, big);
-          __stcg(slot + PA_TILE * (DP + 1) + r, total(r, big));
+          __stcg(slot + HEADS * DP + r, big);
+          __stcg(slot + HEADS * (DP + 1) + r, total(r, big));
         }
       }
     }
@@ -441,16 +490,16 @@ paged_attention_kernel(PagedAttnArgs a, int t0, int n, float* __restrict__ part,
       __syncthreads();
       if (sm_last) {
         __threadfence();
-        auto from = [&](int k) { return part + ((long long)k * 2 + (k == c0 ? 1 : 0)) * PART; };
+        auto from = [&](int k) { return part + ((long long)k * 2 + (k == c0 ? 1 : 0)) * C::PART; };
         for (int i = tid; i < rows * c.D; i += PA_WARPS * 32) {
           const int r = i / c.D, d = i % c.D;
           float big = -CUDART_INF_F, x = 0.f, l = 0.f;
-          for (int k = c0; k <= c1; ++k) big = fmaxf(big, __ldcg(from(k) + PA_TILE * DP + r));
+          for (int k = c0; k <= c1; ++k) big = fmaxf(big, __ldcg(from(k) + HEADS * DP + r));
           for (int k = c0; k <= c1; ++k) {
             const float* p = from(k);
-            const float f = factor(__ldcg(p + PA_TILE * DP + r), big);
+            const float f = factor(__ldcg(p + HEADS * DP + r), big);
             x = fmaf(__ldcg(p + r * DP + d), f, x);
-            l = fmaf(__ldcg(p + PA_TILE * (DP + 1) + r), f, l);
+            l = fmaf(__ldcg(p + HEADS * (DP + 1) + r), f, l);
           }
           put(out + r * a.o_sh + d, l == 0.f ? 0.f : x / l);
         }
@@ -461,58 +510,50 @@ paged_attention_kernel(PagedAttnArgs a, int t0, int n, float* __restrict__ part,
   cp_wait<0>();
 }
 
-int occupancy_of(const void* kern, int smem) {
-  int n = 0;
-  RT_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  RT_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, PA_WARPS * 32, smem));
-  return n < 1 ? 1 : n;
-}
-
-template <typename T, int DP>
+template <typename T, int DP, int NH>
 int ctas_per_sm(int device) {
   static int occ[64] = {0};
-  if (!occ[device]) occ[device] = occupancy_of((const void*)paged_attention_kernel<T, DP>, Cfg<T, DP>::SMEM);
+  if (!occ[device]) {
+    int n = 0;
+    RT_CUDA_CHECK(cudaFuncSetAttribute((const void*)paged_attention_kernel<T, DP, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DP, NH>::SMEM));
+    RT_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_attention_kernel<T, DP, NH>, PA_WARPS * 32, Cfg<DP, NH>::SMEM));
+    RT_CHECK(n >= 1, "paged_attention: the kernel does not fit an SM");
+    occ[device] = n;
+  }
   return occ[device];
 }
 
-template <typename T, int DP>
-struct Run {
-  static void go(const PagedAttnArgs& a, int grid, void* workspace, cudaStream_t s) {
-    int* counters = reinterpret_cast<int*>(workspace);
-    float* part = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + PAGED_ATTN_COUNTER_BYTES);
-    for (int t0 = 0; t0 < a.n_tok; t0 += PAGED_ATTN_CHUNK) {
-      launch_pdl(paged_attention_kernel<T, DP>, dim3(grid), dim3(PA_WARPS * 32), Cfg<T, DP>::SMEM, s, a, t0,
-                 a.n_tok - t0 < PAGED_ATTN_CHUNK ? a.n_tok - t0 : PAGED_ATTN_CHUNK, part, counters, status_word(current_device()));
-      RT_LAUNCH_CHECK();
-    }
-  }
-};
-
-template <typename F> auto by_width(int D, F f) {
-  if (D <= 32) return f(std::integral_constant<int, 32>());
-  if (D <= 64) return f(std::integral_constant<int, 64>());
-  if (D <= 96) return f(std::integral_constant<int, 96>());
-  if (D <= 128) return f(std::integral_constant<int, 128>());
-  if (D <= 192) return f(std::integral_constant<int, 192>());
-  return f(std::integral_constant<int, 256>());
+template <typename F, int DP> auto by_heads(const PagedAttnArgs& a, F f, std::integral_constant<int, DP> dp) {
+  const bool one = a.H / a.cache.Hkv <= 8;
+  if (a.dtype == DT_F16) return one ? f(__half(), dp, std::integral_constant<int, 1>()) : f(__half(), dp, std::integral_constant<int, 2>());
+  return one ? f(__nv_bfloat16(), dp, std::integral_constant<int, 1>()) : f(__nv_bfloat16(), dp, std::integral_constant<int, 2>());
+}
+template <typename F> auto dispatch(const PagedAttnArgs& a, F f) {
+  const int D = a.cache.D;
+  if (D <= 32) return by_heads(a, f, std::integral_constant<int, 32>());
+  if (D <= 64) return by_heads(a, f, std::integral_constant<int, 64>());
+  if (D <= 96) return by_heads(a, f, std::integral_constant<int, 96>());
+  if (D <= 128) return by_heads(a, f, std::integral_constant<int, 128>());
+  if (D <= 192) return by_heads(a, f, std::integral_constant<int, 192>());
+  return by_heads(a, f, std::integral_constant<int, 256>());
 }
 
 }  // namespace
 
 PagedAttnPlan paged_attention_plan(const PagedAttnArgs& a) {
   const int dev = current_device();
-  return by_width(a.cache.D, [&](auto dp) {
-    constexpr int DP = decltype(dp)::value;
-    const int occ = a.dtype == DT_F16 ? ctas_per_sm<__half, DP>(dev) : ctas_per_sm<__nv_bfloat16, DP>(dev);
+  return dispatch(a, [&](auto type, auto dp, auto nh) {
+    constexpr int DP = decltype(dp)::value, NH = decltype(nh)::value;
+    const long long ctas = (long long)ctas_per_sm<decltype(type), DP, NH>(dev) * sm_count(dev);
     // no more CTAs than the longest lengths the table allows could use
     const int G = a.H / a.cache.Hkv;
     long long longest = (long long)a.cache.max_pages * a.cache.page;
     if (a.window > 0 && longest > a.window) longest = a.window;
-    const long long most = (long long)(a.n_tok < PAGED_ATTN_CHUNK ? a.n_tok : PAGED_ATTN_CHUNK) * a.cache.Hkv * ((G + PA_TILE - 1) / PA_TILE) *
+    const long long most = (long long)std::min(a.n_tok, PAGED_ATTN_CHUNK) * a.cache.Hkv * ((G + 8 * NH - 1) / (8 * NH)) *
                            ((longest + PA_UNIT - 1) / PA_UNIT);
     PagedAttnPlan p;
-    p.grid = (int)std::max(1ll, std::min<long long>((long long)occ * sm_count(dev), most));
-    p.workspace_bytes = PAGED_ATTN_COUNTER_BYTES + (long long)occ * sm_count(dev) * 2 * PA_TILE * (DP + 2) * 4;
+    p.grid = (int)std::max(1ll, std::min(ctas, most));
+    p.workspace_bytes = PAGED_ATTN_COUNTER_BYTES + ctas * 2 * Cfg<DP, NH>::PART * 4;
     return p;
   });
 }
@@ -520,10 +561,20 @@ PagedAttnPlan paged_attention_plan(const PagedAttnArgs& a) {
 void paged_attention(const PagedAttnArgs& a, const PagedAttnPlan& p, void* workspace, cudaStream_t s) {
   if (a.n_tok == 0) return;
   RT_CHECK(a.cache.D % 8 == 0 && a.cache.D <= 256 && p.grid * 4 <= PAGED_ATTN_COUNTER_BYTES, "paged_attention: unsupported sizes");
-  by_width(a.cache.D, [&](auto dp) {
-    constexpr int DP = decltype(dp)::value;
-    if (a.dtype == DT_F16) Run<__half, DP>::go(a, p.grid, workspace, s);
-    else Run<__nv_bfloat16, DP>::go(a, p.grid, workspace, s);
+  int* counters = reinterpret_cast<int*>(workspace);
+  float* part = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + PAGED_ATTN_COUNTER_BYTES);
+  int* status = status_word(current_device());
+  // j / page for j < 2^31 as umulhi(2 j, mul) >> shift: with page <= 2^shift the product is off by less than j page / 2^(31 + shift) < 1
+  int shift = 0;
+  while ((1ll << shift) < a.cache.page) ++shift;
+  const unsigned mul = (unsigned)((1ull << (31 + shift)) / (unsigned)a.cache.page + 1);
+  dispatch(a, [&](auto type, auto dp, auto nh) {
+    constexpr int DP = decltype(dp)::value, NH = decltype(nh)::value;
+    for (int t0 = 0; t0 < a.n_tok; t0 += PAGED_ATTN_CHUNK) {
+      launch_pdl(paged_attention_kernel<decltype(type), DP, NH>, dim3(p.grid), dim3(PA_WARPS * 32), Cfg<DP, NH>::SMEM, s, a, mul, shift, t0,
+                 std::min(a.n_tok - t0, PAGED_ATTN_CHUNK), part, counters, status);
+      RT_LAUNCH_CHECK();
+    }
     return 0;
   });
 }
