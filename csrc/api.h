@@ -528,7 +528,7 @@ struct PagedAttnArgs {
   int n_tok, H, window;     // window 0: no limit
   float scale, softcap;     // softcap 0: none
 };
-constexpr int PAGED_ATTN_CHUNK = 512;           // tokens of one launch
+constexpr int PAGED_ATTN_CHUNK = 256;           // tokens of one launch
 constexpr int PAGED_ATTN_COUNTER_BYTES = 8192;  // at the start of the workspace: zeros before its first use, left zero by every call
 struct PagedAttnPlan {
   int grid;

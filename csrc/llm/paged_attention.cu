@@ -12,11 +12,13 @@
 // item that lies in one share is finished there; one that was cut leaves (max, sum, output) parts, and whichever CTA
 // arrives last at its counter joins them in share order, so the result does not depend on timing.
 //
-// Inside a CTA each of four warps owns 16 keys of a unit and its own ring of cp.async stages, without block barriers
-// between units; the ring runs on across items.  The products are m16n8k16 with the cache as the 16 rows and eight query
+// Inside a CTA each of four warps owns 16 keys of a unit and its own ring of stages, without block barriers between
+// units; the ring runs on across items.  Rows are copied by cp.async with their 16-byte pieces on neighbouring lanes: over 131072
+// keys (32 heads on 8, D = 128) 92 us and 6.9 TB/s from one length to the next.  The same rows in 64-byte steps on four lanes
+// took 122 us, as one bulk copy each 124 us (the copy engine takes one every 8 cycles, and a tile is 32 of them).  The products are m16n8k16 with the cache as the 16 rows and eight query
 // heads as the columns: S^T = K Q^T (16 keys), O^T += V^T P^T (16 of D).  Decode has 1 to 16 query heads a kv head, a
-// corner of a 128-row tcgen05 tile; here the tensor time is a fraction of the load time.  A lane copies parts of exactly
-// the two key rows whose scores it later holds, so its page look-ups give its mask too.
+// corner of a 128-row tcgen05 tile; here the tensor time is a fraction of the load time.  Rows that are not visible are not
+// copied: a tile that has some masks their scores, and their values too, which may be left-over NaN.
 // Maximum, sum and output are kept in 32 bits.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -51,14 +53,14 @@ template <int DP, int NH> struct Cfg {         // DP: head size rounded up, NH: 
   static constexpr int OFF_Q = STAGES * PA_WARPS * STAGE;
   static constexpr int OFF_ACC = OFF_Q + (STAGES + 1) * QBUF;
   static constexpr int OFF_ML = OFF_ACC + 2 * HEADS * ACC_LD * 4;
-  static constexpr int OFF_TOK = OFF_ML + 2 * PA_WARPS * HEADS * 4;
+  static constexpr int OFF_TOK = OFF_ML + (2 * PA_WARPS + 3) * HEADS * 4;
   static constexpr int SMEM = OFF_TOK + PAGED_ATTN_CHUNK * 20 + 8;
   static constexpr int PART = HEADS * (DP + 2);                // floats of a part: rows, maxima, sums
   static constexpr bool Q_IN_REGS = DP * NH <= 256;
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool full) {  // zero-fills where not full
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(full ? 16 : 0) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -102,25 +104,23 @@ struct Walk {
 
 template <typename T, int DP, int NH>
 __global__ void __launch_bounds__(PA_WARPS * 32)
-paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, int t0, int n, float* __restrict__ part,
+paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, bool out_vec, int t0, int n, float* __restrict__ part,
                        int* __restrict__ counters, int* __restrict__ status) {
   using C = Cfg<DP, NH>;
-  constexpr int S = C::STAGES, CH = DP / 8, CL = CH / 4, KS = DP / 16, NT = DP / 16, HEADS = C::HEADS;
+  constexpr int S = C::STAGES, CH = DP / 8, KS = DP / 16, NT = DP / 16, HEADS = C::HEADS;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ long long sm_scan[PA_WARPS];
   __shared__ int sm_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const PagedCache& c = a.cache;
   const int G = a.H / c.Hkv, RT = (G + HEADS - 1) / HEADS, HR = c.Hkv * RT;
-  const int chunks = c.D >> 3;
   Tokens tk;
   tk.first = reinterpret_cast<long long*>(smem + C::OFF_TOK);
   tk.lo = reinterpret_cast<int*>(tk.first + PAGED_ATTN_CHUNK + 1);
   tk.len = tk.lo + PAGED_ATTN_CHUNK;
   tk.seq = tk.len + PAGED_ATTN_CHUNK;
-  if (c.D != DP) {  // columns that no copy fills
-    for (int i = tid; i < C::OFF_ACC / 16; i += blockDim.x) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
-  }
+  // zeros in the query rows that no head fills and, for head sizes between the compiled ones, in the columns that no copy fills
+  for (int i = (c.D != DP ? 0 : C::OFF_Q / 16) + tid; i < C::OFF_ACC / 16; i += blockDim.x) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
   pdl_launch_dependents();
   pdl_wait();
 
@@ -203,79 +203,70 @@ paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, int t
   }
   Walk cw = ld;
 
-  // ---- loads: lane copies 16-byte chunks lane % 4, + 4, .. of key rows lane / 4 and lane / 4 + 8; pages are looked up one tile ahead
+  // ---- loads: lanes r and r + 16 look up the page of the tile's key r one tile ahead
   const uint32_t sbase = smem_u32(smem);
-  const uint32_t my_stage = sbase + warp * C::STAGE + (lane >> 2) * C::ROW + (lane & 3) * 16;
-  const T* const nothing = (const T*)a.q;  // source address of copies that only write zeros
-  const int ch0 = lane & 3;
-  const T* const kbase = (const T*)c.k + ch0 * 8;
-  const T* const vbase = (const T*)c.v + ch0 * 8;
+  const uint32_t my_stage = sbase + warp * C::STAGE;
+  const int chunks = c.D >> 3;
+  const int r16 = lane & 15;
   long long left = ue - ub;                // units to load
   int ld_items = 0;
   bool ld_new = true;
-  unsigned j0, jn;                         // this lane's first key of the next tile, the sequence's end
+  unsigned j0, jn;                         // this lane's key of the next tile, the sequence's end
   const int* pages;
   long long head_off;
   auto enter_item = [&]() {
     jn = (unsigned)tk.len[ld.t];
-    j0 = (unsigned)tk.lo[ld.t] + (unsigned)ld.v * PA_UNIT + warp * PA_TILE + (lane >> 2);
+    j0 = (unsigned)tk.lo[ld.t] + (unsigned)ld.v * PA_UNIT + warp * PA_TILE + r16;
     pages = c.table + tk.seq[ld.t] * c.table_stride;
     head_off = (long long)(ld.hr / RT) * c.s_head;
   };
-  int pg[2], row[2];
+  int pg = -1, row = 0;
   auto look_up = [&]() {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const unsigned j = j0 + 8 * e;
-      pg[e] = -1;
-      if (j < jn) {
-        const unsigned k = __umulhi(2 * j, page_mul) >> page_shift;  // j / page
-        row[e] = (int)(j - k * c.page);
-        pg[e] = __ldcg(pages + k);
-        if (pg[e] < 0 || pg[e] >= c.n_pages) {
-          pg[e] = -1;
-          atomicCAS(status, 0, RT_ERR_BOUNDS);
-        }
-      }
+    if (j0 < jn) {
+      const unsigned k = __umulhi(2 * j0, page_mul) >> page_shift;  // j0 / page
+      row = (int)(j0 - k * c.page);
+      pg = __ldcg(pages + k);
     }
   };
-  unsigned seen = 0;  // two bits a stage: whether this lane's two keys count
+  unsigned long long masks = 0;  // 16 bits a stage: which of the tile's keys are there
   auto issue = [&](int stage) {
     if (left > 0) {
+      if (pg >= c.n_pages || (pg < 0 && j0 < jn)) {
+        pg = -1;
+        atomicCAS(status, 0, RT_ERR_BOUNDS);
+      }
+      const unsigned valid = __ballot_sync(0xffffffffu, pg >= 0) & 0xffffu;
+      masks = (masks & ~(0xffffull << (16 * stage))) | (unsigned long long)valid << (16 * stage);
+      const uint32_t dst = my_stage + stage * (PA_WARPS * C::STAGE);
+      const long long off = pg * c.s_page + row * c.s_row + head_off;
       if (ld_new) {  // this warp's quarter of the item's query rows
-        const int hk = ld.hr / RT, r0 = (ld.hr - hk * RT) * HEADS;
-        const uint32_t qd = sbase + C::OFF_Q + (ld_items % (S + 1)) * C::QBUF;
+        constexpr int QR = HEADS / PA_WARPS;
+        const int hk = ld.hr / RT, q0 = (ld.hr - hk * RT) * HEADS + warp * QR;
+        const T* const src = (const T*)a.q + (t0 + ld.t) * a.q_st + (long long)(hk * G + q0) * a.q_sh;
+        const uint32_t q_dst = sbase + C::OFF_Q + (ld_items % (S + 1)) * C::QBUF + warp * QR * C::ROW;
 #pragma unroll
-        for (int i = lane; i < HEADS / 4 * CH; i += 32) {
-          const int r = warp * (HEADS / 4) + i / CH, ch = i % CH;
-          const bool ok = r0 + r < G;
-          if (ch < chunks)
-            cp_async16(qd + r * C::ROW + ch * 16, (const T*)a.q + (ok ? (t0 + ld.t) * a.q_st + (long long)(hk * G + r0 + r) * a.q_sh : 0) + ch * 8, ok);
+        for (int i = lane; i < QR * CH; i += 32) {
+          const int r = i / CH, ch = i % CH;
+          if (q0 + r < G && ch < chunks) cp_async16(q_dst + r * C::ROW + ch * 16, src + r * a.q_sh + ch * 8);
         }
         ++ld_items;
       }
-      const bool ok[2] = {pg[0] >= 0, pg[1] >= 0};
-      seen = (seen & ~(3u << (2 * stage))) | ((ok[0] ? 1u : 0u) | (ok[1] ? 2u : 0u)) << (2 * stage);
-      if (__any_sync(0xffffffffu, ok[0] || ok[1])) {
-        const uint32_t dst = my_stage + stage * (PA_WARPS * C::STAGE);
+      if (valid) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const long long off = pg[e] * c.s_page + row[e] * c.s_row + head_off;
-          const T* const ks = ok[e] ? kbase + off : nothing;
-          const T* const vs = ok[e] ? vbase + off : nothing;
-#pragma unroll
-          for (int i = 0; i < CL; ++i)
-            if (ch0 + 4 * i < chunks) {
-              cp_async16(dst + e * 8 * C::ROW + i * 64, ok[e] ? ks + i * 32 : nothing, ok[e]);
-              cp_async16(dst + (PA_TILE + e * 8) * C::ROW + i * 64, ok[e] ? vs + i * 32 : nothing, ok[e]);
-            }
+        for (int i = 0; i < PA_TILE * CH / 32; ++i) {
+          const int r = (i * 32 + lane) / CH, ch = (i * 32 + lane) % CH;
+          const long long o = __shfl_sync(0xffffffffu, off, r) + ch * 8;
+          if ((valid >> r & 1) && ch < chunks) {
+            cp_async16(dst + r * C::ROW + ch * 16, (const T*)c.k + o);
+            cp_async16(dst + (PA_TILE + r) * C::ROW + ch * 16, (const T*)c.v + o);
+          }
         }
       }
       --left;
       ld_new = ld.v + 1 == ld.nu;
       j0 += PA_UNIT;
       step(ld);
-      pg[0] = pg[1] = -1;
+      pg = -1;
       if (left > 0) {
         if (ld_new) enter_item();
         look_up();
@@ -283,7 +274,11 @@ paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, int t
     }
     cp_commit();
   };
-  __syncthreads();  // the zeroed columns are in place
+  auto arrived = []() {  // this warp's copies of the oldest stage
+    cp_wait<S - 1>();
+    __syncwarp();
+  };
+  __syncthreads();  // the zeros are in place
   enter_item();
   look_up();
 #pragma unroll
@@ -295,6 +290,11 @@ paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, int t
   float* acc_buf = reinterpret_cast<float*>(smem + C::OFF_ACC);
   float* sm_m = reinterpret_cast<float*>(smem + C::OFF_ML);
   float* sm_l = sm_m + PA_WARPS * HEADS;
+  float* sm_top = sm_l + PA_WARPS * HEADS;  // of the item: maxima, sums, and the sum's inverse (0 of an empty row)
+  float* sm_sum = sm_top + HEADS;
+  float* sm_inv = sm_sum + HEADS;
+  static_assert(2 * HEADS * C::ACC_LD >= PA_WARPS * 32 * 4, "the join's sums fit the merge buffer");
+  float4* join_buf = reinterpret_cast<float4*>(smem + C::OFF_ACC);
   // ldmatrix lanes: A fragments of K (rows are keys) and, transposed, of V; B fragments of Q
   const uint32_t k_lane = sbase + warp * C::STAGE + ((lane & 7) + ((lane >> 3) & 1) * 8) * C::ROW + (lane >> 4) * 16;
   const uint32_t v_lane = sbase + warp * C::STAGE + (PA_TILE + (lane & 7) + (lane >> 4) * 8) * C::ROW + ((lane >> 3) & 1) * 16;
@@ -314,7 +314,7 @@ paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, int t
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[h][i][0] = o[h][i][1] = o[h][i][2] = o[h][i][3] = 0.f;
     }
-    cp_wait<S - 1>();
+    arrived();
     __syncthreads();  // all four warps' query rows have arrived; the merge buffer is free again
     const uint32_t q_lane = sbase + C::OFF_Q + (item % (S + 1)) * C::QBUF + (lane & 7) * C::ROW + (lane >> 3) * 16;
     if constexpr (C::Q_IN_REGS) {
@@ -323,12 +323,12 @@ paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, int t
 #pragma unroll
         for (int k2 = 0; k2 < KS / 2; ++k2) ldsm4(q_lane + h * 8 * C::ROW + k2 * 64, qf[h][k2]);
     }
-    for (; u < end; ++u) {
-      cp_wait<S - 1>();
-      __syncwarp();
-      const bool ok0 = seen >> (2 * stage) & 1, ok1 = seen >> (2 * stage) & 2;
-      if (__any_sync(0xffffffffu, ok0 || ok1)) {
+    for (bool first = true; u < end; ++u, first = false) {
+      if (!first) arrived();
+      const unsigned mask = (unsigned)(masks >> (16 * stage)) & 0xffffu;
+      if (mask) {
         const uint32_t st = stage * (PA_WARPS * C::STAGE);
+        const bool all = mask == 0xffffu;
         float s[NH][2][4];  // even and odd steps of D, so that two chains of products run at once
 #pragma unroll
         for (int h = 0; h < NH; ++h)
@@ -359,7 +359,7 @@ paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, int t
           for (int e = 0; e < 4; ++e) {
             float x = (s[h][0][e] + s[h][1][e]) * scale2;
             if (a.softcap > 0.f) x = cap2 - 2.f * cap2 / (ex2_approx(x) + 1.f);  // tanh(y) = 1 - 2 / (exp(2y) + 1), error absolute as a score's may be
-            x = (e < 2 ? ok0 : ok1) ? x : -CUDART_INF_F;
+            if (!all && !(mask >> ((lane >> 2) + (e < 2 ? 0 : 8)) & 1)) x = -CUDART_INF_F;
             grow |= x > m[h][e & 1] + PA_SLACK;
             s[h][0][e] = x;
           }
@@ -393,10 +393,19 @@ paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, int t
           p[h][0] = transpose8x8(pack2<T>(s[h][0][0], s[h][0][1]));  // weights enter the product rounded to the values' type
           p[h][1] = transpose8x8(pack2<T>(s[h][0][2], s[h][0][3]));
         }
+        const int kk = 2 * (lane & 3);
+        const uint32_t keep0 = (mask >> kk & 1 ? 0xffffu : 0u) | (mask >> kk & 2 ? 0xffff0000u : 0u);
+        const uint32_t keep1 = (mask >> (kk + 8) & 1 ? 0xffffu : 0u) | (mask >> (kk + 8) & 2 ? 0xffff0000u : 0u);
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
           uint32_t va[4];
           ldsm4_t(v_lane + st + i * 32, va);
+          if (!all) {
+            va[0] &= keep0;
+            va[1] &= keep0;
+            va[2] &= keep1;
+            va[3] &= keep1;
+          }
 #pragma unroll
           for (int h = 0; h < NH; ++h) mma16816<T>(o[h][i], va, p[h][0], p[h][1]);
         }
@@ -456,58 +465,109 @@ paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, int t
             *x = fmaf(*x, g[e & 1], o[h][i][e] * f[e & 1]);
           }
       }
-    }
-    __syncthreads();
-    auto total = [&](int r, float big) {
+    } else if (warp == 2 && lane < HEADS) {
+      const float big = top(lane);
       float x = 0.f;
 #pragma unroll
-      for (int w = 0; w < PA_WARPS; ++w) x += sm_l[w * HEADS + r] * factor(sm_m[w * HEADS + r], big);
-      return x;
-    };
+      for (int w = 0; w < PA_WARPS; ++w) x += sm_l[w * HEADS + lane] * factor(sm_m[w * HEADS + lane], big);
+      sm_top[lane] = big;
+      sm_sum[lane] = x;
+      sm_inv[lane] = x == 0.f ? 0.f : 1.f / x;
+    }
+    __syncthreads();
     T* const out = (T*)a.out + (t0 + t) * a.o_st + (long long)(hk * G + r0) * a.o_sh;
+    auto store = [&](int r, int d, float4 x, float f) {
+      T* const y = out + r * a.o_sh + d;
+      if (out_vec) {
+        *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(x.x * f, x.y * f), pack2<T>(x.z * f, x.w * f));
+      } else {
+        put(y, x.x * f);
+        put(y + 1, x.y * f);
+        put(y + 2, x.z * f);
+        put(y + 3, x.w * f);
+      }
+    };
+    constexpr int D4 = DP / 4;
+    const int quads = rows * D4;
     const bool whole = g0 >= ub && g1 <= ue;
     float* const slot = part + ((long long)blockIdx.x * 2 + (g0 >= ub ? 1 : 0)) * C::PART;
-    for (int i = tid; i < rows * DP; i += PA_WARPS * 32) {
-      const int r = i / DP, d = i % DP;
-      const float x = acc_buf[r * C::ACC_LD + d] + acc_buf[(HEADS + r) * C::ACC_LD + d];
-      if (whole) {
-        const float l = total(r, top(r));
-        if (d < c.D) put(out + r * a.o_sh + d, l == 0.f ? 0.f : x / l);
-      } else {
-        __stcg(slot + r * DP + d, x);
-        if (d == 0) {
-          const float big = top(r);
-          __stcg(slot + HEADS * DP + r, big);
-          __stcg(slot + HEADS * (DP + 1) + r, total(r, big));
-        }
-      }
+    for (int i = tid; i < quads; i += PA_WARPS * 32) {
+      const int r = i / D4, d = i % D4 * 4;
+      if (d >= c.D) continue;
+      const float4 x = *reinterpret_cast<const float4*>(acc_buf + r * C::ACC_LD + d), y = *reinterpret_cast<const float4*>(acc_buf + (HEADS + r) * C::ACC_LD + d);
+      const float4 z = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+      if (whole) store(r, d, z, sm_inv[r]);
+      else __stcg(reinterpret_cast<float4*>(slot + r * DP + d), z);
     }
     if (!whole) {
+      if (tid < rows) {
+        __stcg(slot + HEADS * DP + tid, sm_top[tid]);
+        __stcg(slot + HEADS * (DP + 1) + tid, sm_sum[tid]);
+      }
       const int c0 = (int)(((g0 + 1) * P - 1) / U), c1 = (int)((g1 * P - 1) / U);
       __threadfence();
       __syncthreads();
       if (tid == 0) sm_last = atomicAdd(&counters[c0], 1) == c1 - c0;
       __syncthreads();
       if (sm_last) {
+        // Parts in share order: first the item's maxima and sums, a warp a row with the parts over its lanes; then the weighted
+        // sum, four values a thread, the parts over the threads that are left and eight loads of each in flight.
         __threadfence();
-        auto from = [&](int k) { return part + ((long long)k * 2 + (k == c0 ? 1 : 0)) * C::PART; };
-        for (int i = tid; i < rows * c.D; i += PA_WARPS * 32) {
-          const int r = i / c.D, d = i % c.D;
-          float big = -CUDART_INF_F, x = 0.f, l = 0.f;
-          for (int k = c0; k <= c1; ++k) big = fmaxf(big, __ldcg(from(k) + HEADS * DP + r));
-          for (int k = c0; k <= c1; ++k) {
-            const float* p = from(k);
-            const float f = factor(__ldcg(p + HEADS * DP + r), big);
-            x = fmaf(__ldcg(p + r * DP + d), f, x);
-            l = fmaf(__ldcg(p + HEADS * (DP + 1) + r), f, l);
+        const int parts = c1 - c0 + 1;
+        auto from = [&](int k) { return part + ((long long)(c0 + k) * 2 + (k == 0 ? 1 : 0)) * C::PART; };
+        for (int r = warp; r < rows; r += PA_WARPS) {
+          float big = -CUDART_INF_F, x = 0.f;
+          for (int k = lane; k < parts; k += 32) big = fmaxf(big, __ldcg(from(k) + HEADS * DP + r));
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+          for (int k = lane; k < parts; k += 32) x = fmaf(__ldcg(from(k) + HEADS * (DP + 1) + r), factor(__ldcg(from(k) + HEADS * DP + r), big), x);
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+          if (lane == 0) {
+            sm_top[r] = big;
+            sm_inv[r] = x == 0.f ? 0.f : 1.f / x;
           }
-          put(out + r * a.o_sh + d, l == 0.f ? 0.f : x / l);
+        }
+        __syncthreads();
+        int split = 1;  // threads that share four values
+        while (quads * split * 2 <= PA_WARPS * 32 && split * 2 <= parts) split *= 2;
+        const int group = tid / quads;
+        const int step_q = split > 1 ? quads : PA_WARPS * 32;
+        for (int i = split > 1 ? tid % quads : tid; i < quads; i += step_q) {
+          const int r = i / D4, d = i % D4 * 4;
+          float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (d < c.D && group < split || split == 1) {
+            const float big = sm_top[r];
+#pragma unroll 8
+            for (int k = split > 1 ? group : 0; k < parts; k += split) {
+              const float* p = from(k);
+              const float f = factor(__ldcg(p + HEADS * DP + r), big);
+              const float4 x = __ldcg(reinterpret_cast<const float4*>(p + r * DP + d));
+              z = make_float4(fmaf(x.x, f, z.x), fmaf(x.y, f, z.y), fmaf(x.z, f, z.z), fmaf(x.w, f, z.w));
+            }
+          }
+          if (split == 1) {
+            if (d < c.D) store(r, d, z, sm_inv[r]);
+          } else if (group < split) {
+            join_buf[group * quads + i] = z;
+          }
+          if (split > 1) break;
+        }
+        if (split > 1) {
+          __syncthreads();
+          if (tid < quads && tid % D4 * 4 < c.D) {
+            float4 z = join_buf[tid];
+            for (int g = 1; g < split; ++g) {
+              const float4 x = join_buf[g * quads + tid];
+              z = make_float4(z.x + x.x, z.y + x.y, z.z + x.z, z.w + x.w);
+            }
+            store(tid / D4, tid % D4 * 4, z, sm_inv[tid / D4]);
+          }
         }
         if (tid == 0) counters[c0] = 0;  // for the next launch that uses this workspace
       }
     }
   }
-  cp_wait<0>();
 }
 
 template <typename T, int DP, int NH>
@@ -568,10 +628,11 @@ void paged_attention(const PagedAttnArgs& a, const PagedAttnPlan& p, void* works
   int shift = 0;
   while ((1ll << shift) < a.cache.page) ++shift;
   const unsigned mul = (unsigned)((1ull << (31 + shift)) / (unsigned)a.cache.page + 1);
+  const bool out_vec = a.o_st % 4 == 0 && a.o_sh % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 8 == 0;
   dispatch(a, [&](auto type, auto dp, auto nh) {
     constexpr int DP = decltype(dp)::value, NH = decltype(nh)::value;
     for (int t0 = 0; t0 < a.n_tok; t0 += PAGED_ATTN_CHUNK) {
-      launch_pdl(paged_attention_kernel<decltype(type), DP, NH>, dim3(p.grid), dim3(PA_WARPS * 32), Cfg<DP, NH>::SMEM, s, a, mul, shift, t0,
+      launch_pdl(paged_attention_kernel<decltype(type), DP, NH>, dim3(p.grid), dim3(PA_WARPS * 32), Cfg<DP, NH>::SMEM, s, a, mul, shift, out_vec, t0,
                  std::min(a.n_tok - t0, PAGED_ATTN_CHUNK), part, counters, status);
       RT_LAUNCH_CHECK();
     }
