@@ -13,7 +13,11 @@
 // A cluster of CTAs takes a row and reads it once, into shared memory.  A threshold is found by histograms (counts for top_k,
 // exact weights for top_p): over 384 equal steps of 46 octaves below the maximum, then over 384 steps of the one where the
 // sum crosses; the few members of that step are ranked by a warp, and should they be too many (equal logits) the histograms
-// go on over their keys.  The draw adds kept weights by warp, then by parts of the stretch that holds the target.
+// go on over their keys.  Passes after the first look at a narrow range and skip the rest by comparing floats.  The draw needs
+// each CTA's kept weight, which its part of the first histogram gives but for one step; then only the CTA that holds the
+// target adds by warp, by parts of a warp's stretch, and walks.
+// Bounds: the row's bytes, and one 64-bit exponential a logit where all weights have to be summed (top_p or no filter), about as
+// many cycles as the load.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -44,10 +48,9 @@ __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// NaN counts as minus infinity, -0 as 0: equal values get equal keys.
-__device__ __forceinline__ float clean(float l) { return l == l ? l + 0.f : -CUDART_INF_F; }
-__device__ __forceinline__ unsigned key_of(float l) {
-  const unsigned b = __float_as_uint(l);
+__device__ __forceinline__ float clean(float l) { return fmaxf(l, -CUDART_INF_F); }  // NaN counts as minus infinity
+__device__ __forceinline__ unsigned key_of(float l) {  // in the order of the values; -0 and 0 get one key
+  const unsigned b = __float_as_uint(l + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
@@ -57,12 +60,14 @@ struct alignas(16) Shared {
   u64 part[2][ST_WARPS];                       // reductions by warp, used in turn
   u64 mass[ST_WARPS], fine_mass[ST_WARPS];     // draw: kept weight above the cut, by warp
   unsigned ties[ST_WARPS], fine_ties[ST_WARPS];  // draw: members at the cut, by warp
-  unsigned lo[2][ST_BINS], hi[2][ST_BINS];     // histograms, used in turn: counts in lo, weights in both
-  unsigned list[ST_LIST];                      // keys of a step's members (the first CTA's)
-  int n_list;
+  unsigned lo[2][ST_BINS], hi[2][ST_BINS];     // histograms (the first, and finer ones): counts in lo, weights in both
+  unsigned list[2][ST_LIST];                   // keys of a step's members, for top_k and for top_p (the first CTA's)
+  int n_list[2];
+  u64 cta_mass;                                // draw: of the whole CTA
+  unsigned cta_ties;
   // what one thread finds for its CTA
   u64 found_mass;
-  unsigned found_key, found_count;
+  unsigned found_key;
   int found_bin;
 };
 
@@ -70,24 +75,48 @@ struct alignas(16) Shared {
 // |r| <= ln 2 / 256, where the series to r^4 is off by 1e-15; adding 2^52 rounds to the integer that the low bits then hold.
 struct Weigh {
   float m, per;                                // maximum; histogram steps per unit of the logit
-  double m64, c;                               // 128 log2(e) / T
+  double m64, c, step;                         // 128 log2(e) / T; 1 / per
   const double* table;
-  // steps below the maximum, monotone in l; 0 for the maximum itself, infinities included
-  __device__ __forceinline__ float steps_below(float l) const { return l == m ? 0.f : fminf((m - l) * per, (float)(ST_BINS - 1)); }
-  __device__ __forceinline__ u64 of(float l) const {
-    const double z = ((double)l - m64) * c;
-    const double magic = 6755399441055744.0;   // 1.5 * 2^52
-    const double t = z + magic;
-    const int k = __double2loint(t);
-    const double f = z - (t - magic);
-    constexpr double A = 0.0054152123481245727;  // ln 2 / 128
-    const double q = f * (A + f * (A * A / 2 + f * (A * A * A / 6 + f * (A * A * A * A / 24))));
-    const double two = table[k & (ST_TABLE - 1)];
-    const double sc = __hiloint2double(__double2hiint(two) + ((k >> 7) << 20), __double2loint(two));
-    const u64 w = (u64)__double_as_longlong(fma(sc, q, sc) + 4503599627370496.0) & 0xfffffffffffffull;  // + 2^52
-    return l == m ? (u64)ST_ONE : w;
+  // steps below the maximum, monotone in l; 0 for the maximum itself, also where a product with infinity is none
+  __device__ __forceinline__ float steps_below(float l) const { return fmaxf((m - l) * per, 0.f); }
+  __device__ __forceinline__ bool possible(float l) const { return steps_below(l) < ST_BINS - 1; }
+  template <int N> __device__ __forceinline__ void of(const float (&l)[N], u64 (&w)[N]) const {  // side by side: the chain is long
+    constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52
+    constexpr double A = 0.0054152123481245727;   // ln 2 / 128
+    double f[N], sc[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = ((double)l[e] - m64) * c;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const double t = f[e] + MAGIC;
+      const int k = __double2loint(t);
+      f[e] -= t - MAGIC;
+      const double two = table[k & (ST_TABLE - 1)];
+      sc[e] = __hiloint2double(__double2hiint(two) + ((k >> 7) << 20), __double2loint(two));
+    }
+    double q[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) q[e] = fma(f[e], A * A * A * A / 24, A * A * A / 6);
+#pragma unroll
+    for (int e = 0; e < N; ++e) q[e] = fma(f[e], q[e], A * A / 2);
+#pragma unroll
+    for (int e = 0; e < N; ++e) q[e] = f[e] * fma(f[e], q[e], A);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const u64 v = (u64)__double_as_longlong(fma(sc[e], q[e], sc[e]) + 4503599627370496.0) & 0xfffffffffffffull;  // + 2^52
+      w[e] = l[e] == m ? (u64)ST_ONE : v;
+    }
   }
-  __device__ __forceinline__ u64 operator()(float l) const { return steps_below(l) < ST_BINS - 1 ? of(l) : 0; }
+  __device__ __forceinline__ u64 of(float l) const {
+    const float x[1] = {l};
+    u64 v[1];
+    of(x, v);
+    return v[0];
+  }
+  __device__ __forceinline__ u64 operator()(float l) const { return possible(l) ? of(l) : 0; }
+  // floats around the logits that lie `steps` below the maximum: rounding moves steps_below by 5e-5 at most
+  __device__ __forceinline__ float surely_below(double steps) const { return __double2float_rd(m64 - (steps + 5e-4) * step); }
+  __device__ __forceinline__ float surely_above(double steps) const { return steps <= 0 ? CUDART_INF_F : __double2float_ru(m64 - (steps - 5e-4) * step); }
 };
 
 struct Add {
@@ -126,19 +155,14 @@ __device__ __forceinline__ u64 cluster_all(cg::cluster_group& cl, int nc, Shared
   return warp_all(v, op);
 }
 
-// The CTA's logits to shared memory, cleaned; returns this thread's largest.  Rows may start anywhere: single values up to a
-// 16-byte boundary, 16 bytes at a time from there on; `slice` is placed so that those land on 16 bytes too.
+// The CTA's n logits to shared memory, cleaned: logit i at slice[pad + i], minus infinity on either side up to whole groups of
+// four; returns this thread's largest.  Rows may start anywhere: single values up to a 16-byte boundary (logit `head`),
+// 16 bytes at a time from there on; `pad` puts those on 16 bytes of shared memory too.
 template <typename T>
-__device__ __forceinline__ float load_slice(const T* x, float* slice, int n, int head) {
+__device__ __forceinline__ float load_slice(const T* x, float* slice, int n, int head, int pad, int quads) {
   constexpr int PER = 16 / sizeof(T);
   float top = -CUDART_INF_F;
-  auto one = [&](int i) {
-    const float l = clean(to_f(x[i]));
-    slice[i] = l;
-    top = fmaxf(top, l);
-  };
-  const int vecs = n > head ? (n - head) / PER : 0, tail = head + vecs * PER;
-  if ((int)threadIdx.x < min(head, n)) one(threadIdx.x);
+  const int vecs = n > head ? (n - head) / PER : 0, tail = n > head ? head + vecs * PER : n;
   const uint4* const v = reinterpret_cast<const uint4*>(x + head);
 #pragma unroll 4
   for (int i = threadIdx.x; i < vecs; i += ST_THREADS) {
@@ -151,9 +175,17 @@ __device__ __forceinline__ float load_slice(const T* x, float* slice, int n, int
       top = fmaxf(top, f[k]);
     }
 #pragma unroll
-    for (int k = 0; k < PER; k += 4) *reinterpret_cast<float4*>(slice + head + i * PER + k) = make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]);
+    for (int k = 0; k < PER; k += 4) *reinterpret_cast<float4*>(slice + pad + head + i * PER + k) = make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]);
   }
-  if (n > head && tail + (int)threadIdx.x < n) one(tail + threadIdx.x);
+  // what is left at both ends, a thread each: pad and head, then tail and pad
+  const int front = pad + min(head, n), rest = 4 * quads - pad - tail;
+  if ((int)threadIdx.x < front + rest) {
+    const int j = (int)threadIdx.x < front ? (int)threadIdx.x : pad + tail + (int)threadIdx.x - front;
+    const int i = j - pad;
+    const float l = i >= 0 && i < n ? clean(to_f(x[i])) : -CUDART_INF_F;
+    slice[j] = l;
+    top = fmaxf(top, l);
+  }
   return top;
 }
 
@@ -161,21 +193,23 @@ template <typename T>
 __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs a, int per) {
   extern __shared__ __align__(16) unsigned char dyn[];
   Shared& sm = *reinterpret_cast<Shared*>(dyn);
+  float* const slice = reinterpret_cast<float*>(dyn + sizeof(Shared));
+  const float4* const slice4 = reinterpret_cast<const float4*>(slice);
   cg::cluster_group cl = cg::this_cluster();
   const int nc = cl.num_blocks(), rank = cl.block_rank();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int row = blockIdx.x / nc;
   const int base = rank * per, n = max(0, min(per, a.vocab - base));  // this CTA's logits
   if (tid < ST_TABLE) sm.table[tid] = exp2((double)tid / ST_TABLE) * ST_ONE;
-  if (tid == 0) sm.n_list = 0;
+  if (tid < 2) sm.n_list[tid] = 0;
   pdl_launch_dependents();
   pdl_wait();
 
   // ---- the row and its maximum
   const T* const x = (const T*)a.logits + row * a.ld + base;
-  const int head = (int)((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T));
-  float* const slice = reinterpret_cast<float*>(dyn + sizeof(Shared)) + (4 - head % 4) % 4;
-  const float top = load_slice(x, slice, n, head);
+  const int head = (int)((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T)), pad = (4 - head % 4) % 4;
+  const int quads = (pad + n + 3) / 4;
+  const float top = load_slice(x, slice, n, head, pad, quads);
   int turn = 0;
   const unsigned best = (unsigned)cluster_all(cl, nc, sm, top == -CUDART_INF_F ? 0 : key_of(top), turn, Larger());
   const double T_ = a.temperature_rows ? (double)a.temperature_rows[row] : a.temperature;
@@ -184,8 +218,8 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
   if (best == 0 || !(T_ > 0.0)) {  // no possible token, or the most likely one: the lowest index that holds the maximum
     u64 first = 0;
     if (best != 0)
-      for (int i = tid; i < n && !first; i += ST_THREADS)
-        if (slice[i] == w.m) first = (unsigned)~(base + i);
+      for (int j = tid; j < 4 * quads && !first; j += ST_THREADS)
+        if (slice[j] == w.m) first = (unsigned)~(base + j - pad);
     first = cluster_all(cl, nc, sm, first, turn, Larger());
     if (rank == 0 && tid == 0) a.out[row] = best == 0 ? -1 : (long long)(int)~(unsigned)first;
     cl.sync();  // no CTA leaves while another reads its shared memory
@@ -193,37 +227,56 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
   }
   w.m64 = w.m;
   w.c = 1.4426950408889634074 / T_ * ST_TABLE;
-  w.per = (float)(1.4426950408889634074 / T_ * ((ST_BINS - 1) / ST_OCTAVES));
+  w.per = fmaxf((float)(1.4426950408889634074 / T_ * ((ST_BINS - 1) / ST_OCTAVES)), 1.17549435e-38f);  // times infinity it stays infinity
+  w.step = 1.0 / (double)w.per;
   w.table = sm.table;
   const int top_k = a.top_k_rows ? a.top_k_rows[row] : a.top_k;
   const double top_p = a.top_p_rows ? (double)a.top_p_rows[row] : a.top_p;
-  const u64 min_w = (u64)ceil(fmax(0.0, fmin(a.min_p_rows ? (double)a.min_p_rows[row] : a.min_p, 1.0)) * ST_ONE);
+  const double min_p = fmax(0.0, fmin(a.min_p_rows ? (double)a.min_p_rows[row] : a.min_p, 1.0));
+  const u64 min_w = (u64)ceil(min_p * ST_ONE);
+  // steps down to the weight p of the maximum's, a hundredth too many at most
+  auto steps_to = [](double p) { return fminf(fmaxf(-log2f((float)p) * (float)((ST_BINS - 1) / ST_OCTAVES), 0.f) + 0.01f, ST_BINS - 1.f); };
+  const float min_steps = steps_to(min_p);
   const bool by_count = top_k > 0 && top_k < a.vocab, by_mass = top_p < 1.0;
+  // f(l) for this thread's logits l >= least, where few are
+  auto each = [&](float least, auto f) {
+#pragma unroll 2
+    for (int q = tid; q < quads; q += ST_THREADS) {
+      const float4 l = slice4[q];
+      if (fmaxf(fmaxf(l.x, l.y), fmaxf(l.z, l.w)) < least) continue;
+      if (l.x >= least) f(l.x);
+      if (l.y >= least) f(l.y);
+      if (l.z >= least) f(l.z);
+      if (l.w >= least) f(l.w);
+    }
+  };
 
   float cut = -CUDART_INF_F;  // kept: logits above the cut, and the first `ties` that equal it
   unsigned ties = 0;
+  const float least_possible = w.surely_below(ST_BINS - 1);
   if (by_count || by_mass) {
-    int h = 0;  // histogram in use
-    auto clear = [&]() {
+    auto clear = [&](int h) {
       sm.lo[h][tid] = sm.hi[h][tid] = 0;
       __syncthreads();
     };
-    auto put = [&](int b, u64 v) {
+    auto put = [&](int h, int b, u64 v) {
       const unsigned low = (unsigned)v, old = atomicAdd(&sm.lo[h][b], low);
       const unsigned high = (unsigned)(v >> 32) + (old + low < old);
       if (high) atomicAdd(&sm.hi[h][b], high);
     };
-    // The first bin at which the running sum over the cluster's histograms reaches `want`, -1: none.  The sum before it is added to
-    // `before`.  Switches to the other histogram: this one is written again a cluster barrier after all have read it.
-    auto crossing = [&](bool mass, u64 want, u64& before) {
-      u64 v = 0;
+    // The first bin at which the running sum over the cluster's histograms h reaches `want`, -1: none.  The sum before it is added to
+    // `before`.
+    auto crossing = [&](int h, bool mass, u64 want, u64& before) {
+      unsigned lo[ST_MAX_CLUSTER], hi[ST_MAX_CLUSTER];
 #pragma unroll
       for (int r = 0; r < ST_MAX_CLUSTER; ++r) {
-        if (r >= nc) break;
-        const Shared* const o = cl.map_shared_rank(&sm, r);
-        v += o->lo[h][tid];
-        if (mass) v += (u64)o->hi[h][tid] << 32;
+        const Shared* const o = cl.map_shared_rank(&sm, r < nc ? r : 0);
+        lo[r] = r < nc ? o->lo[h][tid] : 0;
+        hi[r] = r < nc && mass ? o->hi[h][tid] : 0;
       }
+      u64 v = 0;
+#pragma unroll
+      for (int r = 0; r < ST_MAX_CLUSTER; ++r) v += ((u64)hi[r] << 32) + lo[r];
       u64 run = warp_before(v, lane);
       if (lane == 31) sm.mass[warp] = run + v;
       if (tid == 0) sm.found_bin = -1;
@@ -237,7 +290,6 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
       __syncthreads();
       const int bin = sm.found_bin;
       if (bin >= 0) before = sm.found_mass;
-      h ^= 1;
       __syncthreads();
       return bin;
     };
@@ -246,29 +298,30 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
     auto narrow = [&](bool mass, u64 want, int bin, u64& before) {
       auto sub_step = [&](float l) {  // -1: not a member
         const float t = w.steps_below(l);
-        return (int)t == bin ? (int)((t - bin) * ST_BINS) : -1;
+        return t < ST_BINS - 1 && (int)t == bin ? (int)((t - bin) * ST_BINS) : -1;
       };
-      clear();
-#pragma unroll 4
-      for (int i = tid; i < n; i += ST_THREADS) {
-        const float l = slice[i];
+      float least = w.surely_below(bin + 1), most = w.surely_above(bin);
+      clear(1);
+      each(least, [&](float l) {
+        if (l > most) return;
         const int s = sub_step(l);
-        if (s < 0) continue;
-        if (mass) put(s, w.of(l));
-        else atomicAdd(&sm.lo[h][s], 1u);
-      }
+        if (s < 0) return;
+        if (mass) put(1, s, w.of(l));
+        else atomicAdd(&sm.lo[1][s], 1u);
+      });
       cl.sync();
-      const int sub = crossing(mass, want, before);
+      const int sub = crossing(1, mass, want, before);
       Shared* const first = cl.map_shared_rank(&sm, 0);
-#pragma unroll 4
-      for (int i = tid; i < n; i += ST_THREADS) {
-        const float l = slice[i];
-        if (sub_step(l) != sub) continue;
-        const int k = atomicAdd(&first->n_list, 1);
-        if (k < ST_LIST) first->list[k] = key_of(l);
-      }
+      const int which = mass ? 1 : 0;
+      least = w.surely_below(bin + (sub + 1.0) / ST_BINS);
+      most = w.surely_above(bin + (double)sub / ST_BINS);
+      each(least, [&](float l) {
+        if (l > most || sub_step(l) != sub) return;
+        const int k = atomicAdd(&first->n_list[which], 1);
+        if (k < ST_LIST) first->list[which][k] = key_of(l);
+      });
       cl.sync();
-      const int members = first->n_list;
+      const int members = first->n_list[which];
       if (members <= ST_LIST) {
         if (warp == 0) {
           // a lane weighs up to two members against all
@@ -276,7 +329,7 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
           u64 v[2], over[2] = {before, before}, eq[2] = {0, 0};
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            k[e] = lane + 32 * e < members ? first->list[lane + 32 * e] : 0;
+            k[e] = lane + 32 * e < members ? first->list[which][lane + 32 * e] : 0;
             v[e] = k[e] == 0 ? 0 : mass ? w(of_key(k[e])) : 1;
           }
           for (int j = 0; j < members; ++j) {
@@ -297,53 +350,39 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
         }
         __syncthreads();
         before = sm.found_mass;
-        const unsigned key = sm.found_key;
-        cl.sync();  // the list may be filled again
-        if (rank == 0 && tid == 0) sm.n_list = 0;
-        cl.sync();
-        return of_key(key);
+        return of_key(sm.found_key);
       }
-      // Many members in so narrow a step are equal ones, or nearly so.  Histograms over their keys, whose bounds are the bin's,
-      // a hundredth of a bin wider than rounding could move them.
-      const double high = (double)w.m - (bin - 0.01) / (double)w.per, low = (double)w.m - (bin + 1.01) / (double)w.per;
-      unsigned k_hi = best, k_lo = key_of(clean(__double2float_rd(low)));
-      if (bin > 0) k_hi = min(k_hi, key_of(clean(__double2float_ru(high))));
+      // Many members in so narrow a step are equal ones, or nearly so: histograms over their keys, until a step is one key.
+      unsigned k_hi = min(best, key_of(most)), k_lo = key_of(clean(least));
       while (true) {
         int shift = 0;
         while (((k_hi - k_lo) >> shift) >= ST_BINS) ++shift;
-        clear();
-        for (int i = tid; i < n; i += ST_THREADS) {
-          const float l = slice[i];
+        cl.sync();  // the last histogram has been read
+        clear(1);
+        each(least, [&](float l) {
           const unsigned k = key_of(l);
-          if (k >= k_lo && k <= k_hi && sub_step(l) == sub) {
-            if (mass) put((k_hi - k) >> shift, w.of(l));
-            else atomicAdd(&sm.lo[h][(k_hi - k) >> shift], 1u);
-          }
-        }
+          if (k < k_lo || k > k_hi || sub_step(l) != sub) return;
+          if (mass) put(1, (k_hi - k) >> shift, w.of(l));
+          else atomicAdd(&sm.lo[1][(k_hi - k) >> shift], 1u);
+        });
         cl.sync();
-        if (rank == 0 && tid == 0) sm.n_list = 0;
-        const int s = crossing(mass, want, before);
+        const int s = crossing(1, mass, want, before);
         k_hi -= (unsigned)max(s, 0) << shift;  // a sum that reaches `want` among these members does so in one of their steps
-        if (shift == 0) break;
+        if (shift == 0) return of_key(k_hi);
         k_lo = max(k_lo, k_hi - ((1u << shift) - 1));
       }
-      cl.sync();
-      return of_key(k_hi);
     };
 
-    // Without top_k, weights below (1 - top_p) / (2 vocab) cannot be where top_p is reached: all of them together weigh less than the rest.
-    const u64 floor_w = by_count || !(top_p > 0.0) ? 0 : (u64)((1.0 - top_p) / a.vocab * (0.5 * ST_ONE));
     u64 total = 0, before = 0;
     bool counted = false;
+    clear(0);
     if (by_count) {
-      clear();
-#pragma unroll 4
-      for (int i = tid; i < n; i += ST_THREADS) {
-        const int b = (int)w.steps_below(slice[i]);
-        if (b < ST_BINS - 1) atomicAdd(&sm.lo[h][b], 1u);
-      }
+      each(least_possible, [&](float l) {
+        const int b = (int)w.steps_below(l);
+        if (b < ST_BINS - 1) atomicAdd(&sm.lo[0][b], 1u);
+      });
       cl.sync();
-      const int bin = crossing(false, (u64)top_k, before);
+      const int bin = crossing(0, false, (u64)top_k, before);
       if (bin >= 0) {  // else every possible token is among the first top_k
         cut = narrow(false, (u64)top_k, bin, before);
         ties = (unsigned)((u64)top_k - before);
@@ -351,29 +390,39 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
       }
     }
     if (by_mass) {
-      clear();
-#pragma unroll 2
-      for (int i = tid; i < n; i += ST_THREADS) {
-        const float l = slice[i];
-        const float t = w.steps_below(l);
-        if (t >= ST_BINS - 1 || l < cut) continue;
-        const u64 v = w.of(l);
-        if (l > cut) total += v;
-        if (v > floor_w) put((int)t, v);
+      // Without top_k, weights below (1 - top_p) / (2 vocab) cannot be where top_p is reached: all of them together weigh less than the rest.
+      const double floor_p = by_count ? 0.0 : (1.0 - fmax(top_p, 0.0)) / a.vocab * 0.5;
+      const float floor_l = w.surely_below(steps_to(floor_p));
+      if (by_count) {
+        if (!counted) cl.sync();  // the counts have been read
+        clear(0);
+      }
+      for (int q = tid; q < quads; q += ST_THREADS) {
+        const float4 l4 = slice4[q];
+        const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+        u64 v[4];
+        w.of(l, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float t = w.steps_below(l[e]);
+          if (!(t < ST_BINS - 1) || l[e] < cut) continue;
+          if (l[e] > cut) total += v[e];
+          if (l[e] >= floor_l) put(0, (int)t, v[e]);
+        }
       }
       total = cluster_all(cl, nc, sm, total, turn, Add());
       if (counted) total += ties * w(cut);
-      const double part = ceil((top_p > 0.0 ? top_p : 0.0) * (double)total);
-      const u64 want = part >= 1.0 ? (part < (double)total ? (u64)part : total) : 1;
+      const double some = ceil((top_p > 0.0 ? top_p : 0.0) * (double)total);
+      const u64 want = some >= 1.0 ? (some < (double)total ? (u64)some : total) : 1;
       before = 0;
-      const int bin = crossing(true, want, before);
+      const int bin = crossing(0, true, want, before);
       if (bin >= 0) {  // else every token above the cut is needed
         const float at = narrow(true, want, bin, before);
         const u64 v = w(at);
-        const unsigned some = (unsigned)((want - before + v - 1) / v);
-        if (at > cut || some < ties) {
+        const unsigned now = (unsigned)((want - before + v - 1) / v);
+        if (at > cut || now < ties) {
           cut = at;
-          ties = some;
+          ties = now;
         }
       }
     }
@@ -383,19 +432,26 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
   // part that holds it is walked.
   const u64 cut_w = ties ? w(cut) : 0;
   const bool cut_in = cut_w != 0 && cut_w >= min_w;
+  const float least = fmaxf(fmaxf(cut, least_possible), w.surely_below(min_steps));
   auto over_cut = [&](float l) -> u64 {  // weight of a logit above the cut, 0 where min_p takes it out
-    if (!(l > cut) || !(w.steps_below(l) < ST_BINS - 1)) return 0;
+    if (!(l > cut) || !(l >= least) || !w.possible(l)) return 0;
     const u64 v = w.of(l);
     return v >= min_w ? v : 0;
   };
-  auto stretch = [&](int s0, int s1, u64* mass, unsigned* equal) {
+  auto stretch = [&](int j0, int j1, u64* mass, unsigned* equal) {  // whole groups of four
     u64 m = 0;
     unsigned eq = 0;
-#pragma unroll 4
-    for (int i = s0 + lane; i < s1; i += 32) {
-      const float l = slice[i];
-      m += over_cut(l);
-      eq += l == cut;
+    for (int q = j0 / 4 + lane; q < j1 / 4; q += 32) {
+      const float4 l4 = slice4[q];
+      const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+      if (fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) < least) continue;
+      u64 v[4];
+      w.of(l, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (l[e] > cut && l[e] >= least && w.possible(l[e]) && v[e] >= min_w) m += v[e];
+        eq += l[e] == cut;
+      }
     }
     m = warp_all(m, Add());
     eq = warp_all(eq, Add());
@@ -404,80 +460,83 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
       *equal = eq;
     }
   };
-  const int seg = (per + ST_THREADS - 1) / ST_THREADS * 32;
-  stretch(min(n, warp * seg), min(n, warp * seg + seg), &sm.mass[warp], &sm.ties[warp]);
+  const int end = 4 * quads, seg = ((per + 3 + ST_WARPS - 1) / ST_WARPS + 127) / 128 * 128;
+  // steps of the first histogram that are kept whole: above the cut's, and the one before min_p's
+  const int whole = by_mass && ties ? min((int)w.steps_below(cut), (int)min_steps - 1) : 0;
+  if (whole > 0) {
+    u64 m = tid < whole ? ((u64)sm.hi[0][tid] << 32) + sm.lo[0][tid] : 0;
+    unsigned eq = 0;
+    const float most = w.surely_above(whole);
+    each(least, [&](float l) {
+      if (l > most) return;
+      if (l == cut) ++eq;
+      else if (w.steps_below(l) >= whole) m += over_cut(l);
+    });
+    m = warp_all(m, Add());
+    eq = warp_all(eq, Add());
+    if (lane == 0) {
+      sm.mass[warp] = m;
+      sm.ties[warp] = eq;
+    }
+  } else {
+    stretch(min(end, warp * seg), min(end, warp * seg + seg), &sm.mass[warp], &sm.ties[warp]);
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const u64 m = warp_all(lane < ST_WARPS ? sm.mass[lane] : 0, Add());
+    const unsigned eq = warp_all(lane < ST_WARPS ? sm.ties[lane] : 0, Add());
+    if (lane == 0) {
+      sm.cta_mass = m;
+      sm.cta_ties = eq;
+    }
+  }
   cl.sync();
   double u = a.uniform_f64 ? ((const double*)a.uniform)[row] : (double)((const float*)a.uniform)[row];
   u = u > 0.0 ? u : 0.0;
-  int mine = -1;       // the target's stretch, where it is this CTA's
-  u64 left = 0;        // target minus the kept weight before it
-  unsigned tie = 0;    // members at the cut before it
-  {
-    // all stretches of the row in order, three a lane; every warp does the same
-    constexpr int PER = (ST_MAX_CLUSTER * ST_WARPS + 31) / 32;
-    u64 m[PER], all = 0;
-    unsigned t[PER], sum_t = 0;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int k = lane * PER + e;
-      const bool there = k < nc * ST_WARPS;
-      const Shared* const o = cl.map_shared_rank(&sm, there ? k / ST_WARPS : 0);
-      m[e] = there ? o->mass[k % ST_WARPS] : 0;
-      t[e] = there ? o->ties[k % ST_WARPS] : 0;
-      sum_t += t[e];
+  // a lane a CTA of the row; every warp does the same
+  const Shared* const o = cl.map_shared_rank(&sm, lane < nc ? lane : 0);
+  u64 m = lane < nc ? o->cta_mass : 0;
+  const unsigned eq = lane < nc ? o->cta_ties : 0;
+  unsigned tie = warp_before(eq, lane);  // members at the cut before
+  if (cut_in && tie < ties) m += min(eq, ties - tie) * cut_w;
+  u64 left = warp_before(m, lane);
+  const u64 target = __umul64hi(u < 1.0 ? (u64)(u * 18446744073709551616.0) : ~0ull, __shfl_sync(0xffffffffu, left + m, 31));
+  const unsigned hit = __ballot_sync(0xffffffffu, target >= left && target < left + m);
+  left = target - __shfl_sync(0xffffffffu, left, rank);  // what remains before the target within this CTA, if it is here
+  tie = __shfl_sync(0xffffffffu, tie, rank);
+  if (hit >> rank & 1) {
+    if (whole > 0) {
+      __syncthreads();
+      stretch(min(end, warp * seg), min(end, warp * seg + seg), &sm.mass[warp], &sm.ties[warp]);
+      __syncthreads();
     }
-    unsigned run_t = warp_before(sum_t, lane);
-    unsigned before_t[PER];
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      before_t[e] = run_t;
-      if (cut_in && run_t < ties) m[e] += min(t[e], ties - run_t) * cut_w;
-      run_t += t[e];
-      all += m[e];
-    }
-    u64 run = warp_before(all, lane);
-    const u64 sum = __shfl_sync(0xffffffffu, run + all, 31);
-    const u64 target = __umul64hi(u < 1.0 ? (u64)(u * 18446744073709551616.0) : ~0ull, sum);
-    int hit = -1;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      if (target >= run && target < run + m[e]) {
-        hit = lane * PER + e;
-        left = target - run;
-        tie = before_t[e];
+    auto find = [&](const u64* mass, const unsigned* equal) {  // the part that holds the target
+      int k = 0;
+      for (; k < ST_WARPS - 1; ++k) {
+        const u64 v = mass[k] + (cut_in && tie < ties ? min(equal[k], ties - tie) * cut_w : 0);
+        if (left < v) break;
+        left -= v;
+        tie += equal[k];
       }
-      run += m[e];
-    }
-    const int from = __ffs(__ballot_sync(0xffffffffu, hit >= 0)) - 1;
-    hit = __shfl_sync(0xffffffffu, hit, from);
-    left = __shfl_sync(0xffffffffu, left, from);
-    tie = __shfl_sync(0xffffffffu, tie, from);
-    if (hit / ST_WARPS == rank) mine = hit % ST_WARPS;
-  }
-  if (mine >= 0) {
-    const int s0 = min(n, mine * seg), s1 = min(n, s0 + seg), fine = (seg + ST_THREADS - 1) / ST_THREADS * 32;
-    stretch(min(s1, s0 + warp * fine), min(s1, s0 + warp * fine + fine), &sm.fine_mass[warp], &sm.fine_ties[warp]);
+      return k;
+    };
+    const int j0 = min(end, find(sm.mass, sm.ties) * seg), j1 = min(end, j0 + seg), fine = ((seg + ST_WARPS - 1) / ST_WARPS + 31) / 32 * 32;
+    stretch(min(j1, j0 + warp * fine), min(j1, j0 + warp * fine + fine), &sm.fine_mass[warp], &sm.fine_ties[warp]);
     __syncthreads();
-    int part = 0;
-    for (; part < ST_WARPS - 1; ++part) {
-      const u64 m = sm.fine_mass[part] + (cut_in && tie < ties ? min(sm.fine_ties[part], ties - tie) * cut_w : 0);
-      if (left < m) break;
-      left -= m;
-      tie += sm.fine_ties[part];
-    }
-    if (part == warp) {
-      const int e = min(s1, s0 + part * fine + fine);
-      for (int i0 = s0 + part * fine; i0 < e; i0 += 32) {
-        const int i = i0 + lane;
-        const float l = i < e ? slice[i] : CUDART_NAN_F;
+    const int k = find(sm.fine_mass, sm.fine_ties);
+    if (k == warp) {
+      const int e = min(j1, j0 + k * fine + fine);
+      for (int i0 = j0 + k * fine; i0 < e; i0 += 32) {
+        const int j = i0 + lane;
+        const float l = j < e ? slice[j] : CUDART_NAN_F;
         const unsigned eqs = __ballot_sync(0xffffffffu, l == cut);
         u64 v = over_cut(l);
         if (l == cut && cut_in && tie + __popc(eqs & ((1u << lane) - 1)) < ties) v = cut_w;
         tie += __popc(eqs);
         const u64 run = warp_before(v, lane) + v;
-        const unsigned hit = __ballot_sync(0xffffffffu, run > left);
-        if (hit) {
-          if (lane == __ffs(hit) - 1) a.out[row] = base + i;
+        const unsigned here = __ballot_sync(0xffffffffu, run > left);
+        if (here) {
+          if (lane == __ffs(here) - 1) a.out[row] = base + j - pad;
           break;
         }
         left -= __shfl_sync(0xffffffffu, run, 31);
@@ -494,7 +553,7 @@ void launch(const SampleArgs& a, cudaStream_t s) {
   while (nc < ST_MAX_CLUSTER && (a.vocab + nc - 1) / nc > 8192) nc *= 2;
   while (nc < ST_MAX_CLUSTER && (long long)a.rows * nc * 2 <= sm_count(current_device()) && a.vocab / nc > 2048) nc *= 2;
   const int per = (a.vocab + nc - 1) / nc;
-  const int smem = (int)sizeof(Shared) + per * 4 + 16;
+  const int smem = (int)sizeof(Shared) + (per + 6) / 4 * 16;  // a slice and up to three places before it
   static int allowed[64] = {0};
   const int dev = current_device();
   if (smem > allowed[dev]) {
