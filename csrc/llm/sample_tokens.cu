@@ -13,11 +13,10 @@
 // A cluster of CTAs takes a row and reads it once, into shared memory.  A threshold is found by histograms (counts for top_k,
 // exact weights for top_p): over 384 equal steps of 46 octaves below the maximum, then over 384 steps of the one where the
 // sum crosses; the few members of that step are ranked by a warp, and should they be too many (equal logits) the histograms
-// go on over their keys.  Passes after the first look at a narrow range and skip the rest by comparing floats.  The draw needs
-// each CTA's kept weight, which its part of the first histogram gives but for one step; then only the CTA that holds the
-// target adds by warp, by parts of a warp's stretch, and walks.
-// Bounds: the row's bytes, and one 64-bit exponential a logit where all weights have to be summed (top_p or no filter), about as
-// many cycles as the load.
+// go on over their keys.  Members of a crossing step are queued by the one pass that compares floats to find them, and only the queue is
+// looked at again.  The draw needs each CTA's kept weight, which its part of the first histogram and the queue give; then only the
+// CTA that holds the target adds by warp, by parts of a warp's stretch, and walks.
+// Bound by issue slots where all weights are summed (top_p or no filter): a 64-bit exponential is 18 instructions a logit.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -40,6 +39,7 @@ constexpr int ST_THREADS = 384, ST_WARPS = ST_THREADS / 32;  // three CTAs an SM
 constexpr int ST_MAX_CLUSTER = 8;
 constexpr int ST_BINS = ST_THREADS;            // a bin a thread where sums over them are formed
 constexpr int ST_LIST = 64;                    // members of a step that a warp ranks
+constexpr int ST_QUEUE = 512;                  // members of a step that a CTA keeps at hand
 constexpr int ST_TABLE = 128;                  // 2^(i / 128)
 constexpr double ST_ONE = 35184372088832.0;    // 2^45
 constexpr double ST_OCTAVES = 46.0;            // further below the maximum weights are zero
@@ -61,8 +61,9 @@ struct alignas(16) Shared {
   u64 mass[ST_WARPS], fine_mass[ST_WARPS];     // draw: kept weight above the cut, by warp
   unsigned ties[ST_WARPS], fine_ties[ST_WARPS];  // draw: members at the cut, by warp
   unsigned lo[2][ST_BINS], hi[2][ST_BINS];     // histograms (the first, and finer ones): counts in lo, weights in both
-  unsigned list[2][ST_LIST];                   // keys of a step's members, for top_k and for top_p (the first CTA's)
-  int n_list[2];
+  unsigned list[2][ST_LIST];                   // keys of a finer step's members, for top_k and for top_p (the first CTA's)
+  float queue[ST_QUEUE];                       // this CTA's members of the crossing step
+  int n_list[2], n_queue;
   u64 cta_mass;                                // draw: of the whole CTA
   unsigned cta_ties;
   // what one thread finds for its CTA
@@ -92,7 +93,8 @@ struct Weigh {
       const int k = __double2loint(t);
       f[e] -= t - MAGIC;
       const double two = table[k & (ST_TABLE - 1)];
-      sc[e] = __hiloint2double(__double2hiint(two) + ((k >> 7) << 20), __double2loint(two));
+      static_assert(ST_TABLE == 128, "the exponent's share of k, moved from bit 7 to bit 20");
+      sc[e] = __hiloint2double(__double2hiint(two) + (k & ~(ST_TABLE - 1)) * (1 << 13), __double2loint(two));
     }
     double q[N];
 #pragma unroll
@@ -103,8 +105,7 @@ struct Weigh {
     for (int e = 0; e < N; ++e) q[e] = f[e] * fma(f[e], q[e], A);
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      const u64 v = (u64)__double_as_longlong(fma(sc[e], q[e], sc[e]) + 4503599627370496.0) & 0xfffffffffffffull;  // + 2^52
-      w[e] = l[e] == m ? (u64)ST_ONE : v;
+      w[e] = (u64)__double_as_longlong(fma(sc[e], q[e], sc[e]) + 4503599627370496.0) & 0xfffffffffffffull;  // + 2^52
     }
   }
   __device__ __forceinline__ u64 of(float l) const {
@@ -149,8 +150,16 @@ __device__ __forceinline__ u64 cluster_all(cg::cluster_group& cl, int nc, Shared
   v = warp_all(v, op);
   if ((threadIdx.x & 31) == 0) sm.part[turn][threadIdx.x >> 5] = v;
   cl.sync();
-  v = 0;
-  for (int k = threadIdx.x & 31; k < nc * ST_WARPS; k += 32) v = op(v, cl.map_shared_rank(&sm, k / ST_WARPS)->part[turn][k % ST_WARPS]);
+  constexpr int PER = (ST_MAX_CLUSTER * ST_WARPS + 31) / 32;
+  u64 got[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int k = (threadIdx.x & 31) + 32 * e;
+    got[e] = k < nc * ST_WARPS ? cl.map_shared_rank(&sm, k / ST_WARPS)->part[turn][k % ST_WARPS] : 0;
+  }
+  v = got[0];
+#pragma unroll
+  for (int e = 1; e < PER; ++e) v = op(v, got[e]);
   turn ^= 1;
   return warp_all(v, op);
 }
@@ -225,8 +234,14 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
     cl.sync();  // no CTA leaves while another reads its shared memory
     return;
   }
+  if (w.m == CUDART_INF_F) {  // such logits share all the weight: the row becomes 0 for them and minus infinity elsewhere
+    __syncthreads();
+    for (int j = tid; j < 4 * quads; j += ST_THREADS) slice[j] = slice[j] == CUDART_INF_F ? 0.f : -CUDART_INF_F;
+    w.m = 0.f;
+    __syncthreads();
+  }
   w.m64 = w.m;
-  w.c = 1.4426950408889634074 / T_ * ST_TABLE;
+  w.c = fmin(1.4426950408889634074 / T_ * ST_TABLE, 1e300);
   w.per = fmaxf((float)(1.4426950408889634074 / T_ * ((ST_BINS - 1) / ST_OCTAVES)), 1.17549435e-38f);  // times infinity it stays infinity
   w.step = 1.0 / (double)w.per;
   w.table = sm.table;
@@ -240,7 +255,6 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
   const bool by_count = top_k > 0 && top_k < a.vocab, by_mass = top_p < 1.0;
   // f(l) for this thread's logits l >= least, where few are
   auto each = [&](float least, auto f) {
-#pragma unroll 2
     for (int q = tid; q < quads; q += ST_THREADS) {
       const float4 l = slice4[q];
       if (fmaxf(fmaxf(l.x, l.y), fmaxf(l.z, l.w)) < least) continue;
@@ -250,10 +264,34 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
       if (l.w >= least) f(l.w);
     }
   };
+  // the least float from `low` to the maximum that is kept by a test that larger ones pass too; 32 at a time, in every warp
+  auto least_that = [&](float low, auto passes) {
+    unsigned k_lo = key_of(low), k_hi = key_of(w.m);
+    while (k_lo < k_hi) {
+      const unsigned step = (k_hi - k_lo + 31) / 32, k = min(k_hi, k_lo + lane * step);
+      const unsigned ok = __ballot_sync(0xffffffffu, passes(of_key(k)));
+      const int at = ok ? __ffs(ok) - 1 : 32;
+      if (at < 32) k_hi = min(k_hi, k_lo + at * step);
+      if (at > 0) k_lo = min(k_hi, k_lo + (at - 1) * step + 1);
+    }
+    return of_key(k_hi);
+  };
+  const float least_possible = least_that(w.surely_below(ST_BINS - 1), [&](float l) { return w.possible(l); });
 
   float cut = -CUDART_INF_F;  // kept: logits above the cut, and the first `ties` that equal it
   unsigned ties = 0;
-  const float least_possible = w.surely_below(ST_BINS - 1);
+  // f(l) for the members of a step of the first histogram that are in this CTA
+  int step_bin = -1;
+  auto members = [&](auto f) {
+    if (sm.n_queue <= ST_QUEUE) {
+      for (int i = tid; i < sm.n_queue; i += ST_THREADS) f(sm.queue[i]);
+    } else {
+      each(w.surely_below(step_bin + 1), [&](float l) {
+        const float t = w.steps_below(l);
+        if (t < ST_BINS - 1 && (int)t == step_bin) f(l);
+      });
+    }
+  };
   if (by_count || by_mass) {
     auto clear = [&](int h) {
       sm.lo[h][tid] = sm.hi[h][tid] = 0;
@@ -281,8 +319,7 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
       if (lane == 31) sm.mass[warp] = run + v;
       if (tid == 0) sm.found_bin = -1;
       __syncthreads();
-      run += before;
-      for (int k = 0; k < warp; ++k) run += sm.mass[k];
+      run += before + warp_all(lane < warp ? sm.mass[lane] : 0, Add());
       if (run < want && run + v >= want) {
         sm.found_bin = tid;
         sm.found_mass = run;
@@ -296,43 +333,44 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
     // The logit at which the sum reaches `want`, a member of step `bin` of the first histogram; `before` becomes the sum over
     // larger logits.
     auto narrow = [&](bool mass, u64 want, int bin, u64& before) {
-      auto sub_step = [&](float l) {  // -1: not a member
-        const float t = w.steps_below(l);
-        return t < ST_BINS - 1 && (int)t == bin ? (int)((t - bin) * ST_BINS) : -1;
-      };
-      float least = w.surely_below(bin + 1), most = w.surely_above(bin);
+      auto sub_step = [&](float l) { return (int)((w.steps_below(l) - bin) * ST_BINS); };
+      step_bin = bin;
+      const float most = w.surely_above(bin);
+      if (tid == 0) sm.n_queue = 0;
       clear(1);
-      each(least, [&](float l) {
-        if (l > most) return;
-        const int s = sub_step(l);
-        if (s < 0) return;
-        if (mass) put(1, s, w.of(l));
-        else atomicAdd(&sm.lo[1][s], 1u);
+      each(w.surely_below(bin + 1), [&](float l) {
+        const float t = w.steps_below(l);
+        if (l > most || !(t < ST_BINS - 1) || (int)t != bin) return;
+        const int k = atomicAdd(&sm.n_queue, 1);
+        if (k < ST_QUEUE) sm.queue[k] = l;
+      });
+      __syncthreads();
+      members([&](float l) {
+        if (mass) put(1, sub_step(l), w.of(l));
+        else atomicAdd(&sm.lo[1][sub_step(l)], 1u);
       });
       cl.sync();
       const int sub = crossing(1, mass, want, before);
       Shared* const first = cl.map_shared_rank(&sm, 0);
       const int which = mass ? 1 : 0;
-      least = w.surely_below(bin + (sub + 1.0) / ST_BINS);
-      most = w.surely_above(bin + (double)sub / ST_BINS);
-      each(least, [&](float l) {
-        if (l > most || sub_step(l) != sub) return;
+      members([&](float l) {
+        if (sub_step(l) != sub) return;
         const int k = atomicAdd(&first->n_list[which], 1);
         if (k < ST_LIST) first->list[which][k] = key_of(l);
       });
       cl.sync();
-      const int members = first->n_list[which];
-      if (members <= ST_LIST) {
+      const int found = first->n_list[which];
+      if (found <= ST_LIST) {
         if (warp == 0) {
           // a lane weighs up to two members against all
           unsigned k[2];
           u64 v[2], over[2] = {before, before}, eq[2] = {0, 0};
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            k[e] = lane + 32 * e < members ? first->list[which][lane + 32 * e] : 0;
+            k[e] = lane + 32 * e < found ? first->list[which][lane + 32 * e] : 0;
             v[e] = k[e] == 0 ? 0 : mass ? w(of_key(k[e])) : 1;
           }
-          for (int j = 0; j < members; ++j) {
+          for (int j = 0; j < found; ++j) {
             const unsigned kj = __shfl_sync(0xffffffffu, j < 32 ? k[0] : k[1], j & 31);
             const u64 vj = __shfl_sync(0xffffffffu, j < 32 ? v[0] : v[1], j & 31);
 #pragma unroll
@@ -353,13 +391,13 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
         return of_key(sm.found_key);
       }
       // Many members in so narrow a step are equal ones, or nearly so: histograms over their keys, until a step is one key.
-      unsigned k_hi = min(best, key_of(most)), k_lo = key_of(clean(least));
+      unsigned k_hi = min(key_of(w.m), key_of(most)), k_lo = key_of(w.surely_below(bin + 1));
       while (true) {
         int shift = 0;
         while (((k_hi - k_lo) >> shift) >= ST_BINS) ++shift;
         cl.sync();  // the last histogram has been read
         clear(1);
-        each(least, [&](float l) {
+        members([&](float l) {
           const unsigned k = key_of(l);
           if (k < k_lo || k > k_hi || sub_step(l) != sub) return;
           if (mass) put(1, (k_hi - k) >> shift, w.of(l));
@@ -377,10 +415,13 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
     bool counted = false;
     clear(0);
     if (by_count) {
-      each(least_possible, [&](float l) {
-        const int b = (int)w.steps_below(l);
-        if (b < ST_BINS - 1) atomicAdd(&sm.lo[0][b], 1u);
-      });
+      for (int q = tid; q < quads; q += ST_THREADS) {
+        const float4 l4 = slice4[q];
+        const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (l[e] >= least_possible) atomicAdd(&sm.lo[0][(int)w.steps_below(l[e])], 1u);
+      }
       cl.sync();
       const int bin = crossing(0, false, (u64)top_k, before);
       if (bin >= 0) {  // else every possible token is among the first top_k
@@ -397,17 +438,23 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
         if (!counted) cl.sync();  // the counts have been read
         clear(0);
       }
+      const float above = counted ? of_key(key_of(cut) + 1) : least_possible, put_from = fmaxf(fmaxf(cut, least_possible), floor_l);
       for (int q = tid; q < quads; q += ST_THREADS) {
         const float4 l4 = slice4[q];
         const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+        if (fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) < fmaxf(cut, least_possible)) continue;
         u64 v[4];
         w.of(l, v);
+        unsigned old[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float t = w.steps_below(l[e]);
-          if (!(t < ST_BINS - 1) || l[e] < cut) continue;
-          if (l[e] > cut) total += v[e];
-          if (l[e] >= floor_l) put(0, (int)t, v[e]);
+          if (l[e] >= above) total += v[e];
+          old[e] = l[e] >= put_from ? atomicAdd(&sm.lo[0][(int)w.steps_below(l[e])], (unsigned)v[e]) : 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned high = (unsigned)(v[e] >> 32) + (old[e] + (unsigned)v[e] < old[e]);
+          if (l[e] >= put_from && high) atomicAdd(&sm.hi[0][(int)w.steps_below(l[e])], high);
         }
       }
       total = cluster_all(cl, nc, sm, total, turn, Add());
@@ -430,28 +477,25 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
 
   // ---- draw.  A warp's stretch is contiguous; the one that holds the target is cut into a part for each warp of its CTA, and the
   // part that holds it is walked.
-  const u64 cut_w = ties ? w(cut) : 0;
-  const bool cut_in = cut_w != 0 && cut_w >= min_w;
-  const float least = fmaxf(fmaxf(cut, least_possible), w.surely_below(min_steps));
-  auto over_cut = [&](float l) -> u64 {  // weight of a logit above the cut, 0 where min_p takes it out
-    if (!(l > cut) || !(l >= least) || !w.possible(l)) return 0;
-    const u64 v = w.of(l);
-    return v >= min_w ? v : 0;
-  };
+  const float least = min_p > 0.0 ? fmaxf(least_possible, least_that(fmaxf(least_possible, w.surely_below(min_steps)), [&](float l) { return w.of(l) >= min_w; }))
+                                  : least_possible;
+  const u64 cut_w = ties && cut >= least ? w.of(cut) : 0;
+  const bool cut_in = cut_w != 0;
+  const float lower = fmaxf(least, ties ? of_key(key_of(cut) + 1) : least);  // kept: l >= lower, and the cut's
   auto stretch = [&](int j0, int j1, u64* mass, unsigned* equal) {  // whole groups of four
     u64 m = 0;
     unsigned eq = 0;
     for (int q = j0 / 4 + lane; q < j1 / 4; q += 32) {
       const float4 l4 = slice4[q];
       const float l[4] = {l4.x, l4.y, l4.z, l4.w};
-      if (fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) < least) continue;
+      const float top4 = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));
+      if (cut_in) eq += (l[0] == cut) + (l[1] == cut) + (l[2] == cut) + (l[3] == cut);
+      if (top4 < lower) continue;
       u64 v[4];
       w.of(l, v);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (l[e] > cut && l[e] >= least && w.possible(l[e]) && v[e] >= min_w) m += v[e];
-        eq += l[e] == cut;
-      }
+      for (int e = 0; e < 4; ++e)
+        if (l[e] >= lower) m += v[e];
     }
     m = warp_all(m, Add());
     eq = warp_all(eq, Add());
@@ -461,16 +505,14 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
     }
   };
   const int end = 4 * quads, seg = ((per + 3 + ST_WARPS - 1) / ST_WARPS + 127) / 128 * 128;
-  // steps of the first histogram that are kept whole: above the cut's, and the one before min_p's
-  const int whole = by_mass && ties ? min((int)w.steps_below(cut), (int)min_steps - 1) : 0;
+  // steps of the first histogram that are kept whole: those above the cut's, whose members are queued; none where min_p cuts higher
+  const int whole = by_mass && cut_in ? (int)w.steps_below(cut) : 0;
   if (whole > 0) {
     u64 m = tid < whole ? ((u64)sm.hi[0][tid] << 32) + sm.lo[0][tid] : 0;
     unsigned eq = 0;
-    const float most = w.surely_above(whole);
-    each(least, [&](float l) {
-      if (l > most) return;
-      if (l == cut) ++eq;
-      else if (w.steps_below(l) >= whole) m += over_cut(l);
+    members([&](float l) {
+      if (l >= lower) m += w.of(l);
+      eq += l == cut;
     });
     m = warp_all(m, Add());
     eq = warp_all(eq, Add());
@@ -510,14 +552,15 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
       stretch(min(end, warp * seg), min(end, warp * seg + seg), &sm.mass[warp], &sm.ties[warp]);
       __syncthreads();
     }
-    auto find = [&](const u64* mass, const unsigned* equal) {  // the part that holds the target
-      int k = 0;
-      for (; k < ST_WARPS - 1; ++k) {
-        const u64 v = mass[k] + (cut_in && tie < ties ? min(equal[k], ties - tie) * cut_w : 0);
-        if (left < v) break;
-        left -= v;
-        tie += equal[k];
-      }
+    auto find = [&](const u64* mass, const unsigned* equal) {  // the part that holds the target; every warp does the same
+      const unsigned eq = lane < ST_WARPS ? equal[lane] : 0, t = tie + warp_before(eq, lane);
+      u64 v = lane < ST_WARPS ? mass[lane] : 0;
+      if (cut_in && t < ties) v += min(eq, ties - t) * cut_w;
+      const u64 run = warp_before(v, lane);
+      const unsigned in = __ballot_sync(0xffffffffu, left >= run && left < run + v);
+      const int k = in ? __ffs(in) - 1 : 0;
+      left -= __shfl_sync(0xffffffffu, run, k);
+      tie = __shfl_sync(0xffffffffu, t, k);
       return k;
     };
     const int j0 = min(end, find(sm.mass, sm.ties) * seg), j1 = min(end, j0 + seg), fine = ((seg + ST_WARPS - 1) / ST_WARPS + 31) / 32 * 32;
@@ -530,7 +573,7 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
         const int j = i0 + lane;
         const float l = j < e ? slice[j] : CUDART_NAN_F;
         const unsigned eqs = __ballot_sync(0xffffffffu, l == cut);
-        u64 v = over_cut(l);
+        u64 v = l >= lower ? w.of(l) : 0;
         if (l == cut && cut_in && tie + __popc(eqs & ((1u << lane) - 1)) < ties) v = cut_w;
         tie += __popc(eqs);
         const u64 run = warp_before(v, lane) + v;
