@@ -16,14 +16,17 @@ from __future__ import annotations
 import math
 import time
 from dataclasses import dataclass
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, Optional, Tuple, Union
 
 import torch
 import torch.distributed as dist
 
 from .. import _native
 from ..formats import gguf
+from ..ops.paged import paged_append, paged_attention
+from ..ops.sampling import sample_tokens
 from .quant import QuantLinear
+from .sampling import SamplingConfig
 
 
 @dataclass
@@ -77,13 +80,67 @@ class KVCache:
         return sum(t.numel() * t.element_size() for t in self.k + self.v)
 
 
+class PagedKVCache:
+    """Key/value cache in pages ``[n_pages, Hkv_local, page, D]`` per layer that the sequences share: a sequence holds the pages its
+    positions need (``reserve``) and gives them back (``release``), so memory follows the lengths in use instead of
+    ``batch * max_len``.  ``block_table [batch, ceil(max_len / page)]`` (int32, on the device) names a sequence's pages, -1 where
+    it has none.  ``n_pages`` defaults to what ``batch`` sequences of ``max_len`` need."""
+
+    def __init__(self, n_layer: int, batch: int, n_head_kv: int, max_len: int, head_dim: int, device, dtype=torch.float16, page: int = 64,
+                 n_pages: Optional[int] = None):
+        if page < 1 or max_len < 1 or batch < 1:
+            raise ValueError("batch, max_len and page must be at least 1")
+        per_seq = (max_len + page - 1) // page
+        self.n_pages = batch * per_seq if n_pages is None else int(n_pages)
+        self.k = [torch.zeros(self.n_pages, n_head_kv, page, head_dim, dtype=dtype, device=device) for _ in range(n_layer)]
+        self.v = [torch.zeros(self.n_pages, n_head_kv, page, head_dim, dtype=dtype, device=device) for _ in range(n_layer)]
+        self.page, self.max_len = page, max_len
+        self.block_table = torch.full((batch, per_seq), -1, dtype=torch.int32, device=device)
+        self.pages: List[List[int]] = [[] for _ in range(batch)]
+        self.free = list(range(self.n_pages - 1, -1, -1))
+        self.lengths = [0] * batch
+
+    def reserve(self, b: int, length: int) -> None:
+        """Gives sequence ``b`` pages for positions ``0 .. length - 1``; those it has stay."""
+        if length > self.max_len:
+            raise ValueError(f"{length} positions exceed the cache's limit of {self.max_len}")
+        have, need = len(self.pages[b]), (length + self.page - 1) // self.page
+        if need <= have:
+            return
+        if need - have > len(self.free):
+            raise RuntimeError(f"paged cache is full: sequence {b} needs {need - have} more pages, {len(self.free)} of {self.n_pages} are free")
+        new = [self.free.pop() for _ in range(need - have)]
+        self.pages[b] += new
+        self.block_table[b, have:need] = torch.tensor(new, dtype=torch.int32).to(self.block_table.device)
+
+    def release(self, b: int) -> None:
+        """Takes all pages of sequence ``b`` back and forgets its contents."""
+        self.free += reversed(self.pages[b])
+        self.pages[b] = []
+        self.block_table[b].fill_(-1)
+        self.lengths[b] = 0
+
+    def seq_len(self, b: int = 0) -> int:
+        return self.lengths[b]
+
+    def clear(self) -> None:
+        for b in range(len(self.lengths)):
+            self.release(b)
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in self.k + self.v)
+
+
 class _DecodeGraph:
     """Static device tensors and the captured graph of one decode step."""
-    tok = pos = seq = step = out = logits = graph = None
+    tok = pos = seq = step = out = logits = graph = uniform = None
 
 
 class _Layer:
     __slots__ = ("attn_norm", "wqkv", "wo", "ffn_norm", "w_gate_up", "w_down", "qkv_bias")
+
+    def __init__(self):
+        self.qkv_bias = None               # most checkpoints have none
 
 
 class LlamaRuntime:
@@ -285,6 +342,10 @@ class LlamaRuntime:
         return KVCache(self.cfg.n_layer, batch, self.hkv_local, max_len or self.cfg.context_length, self.cfg.head_dim,
                        self.device, self.act_dtype)
 
+    def new_paged_cache(self, batch: int, max_len: Optional[int] = None, page: int = 64, n_pages: Optional[int] = None) -> PagedKVCache:
+        return PagedKVCache(self.cfg.n_layer, batch, self.hkv_local, max_len or self.cfg.context_length, self.cfg.head_dim, self.device,
+                            self.act_dtype, page, n_pages)
+
     # ---------------------------------------------------------------- forward
     def _all_reduce(self, x: torch.Tensor) -> torch.Tensor:
         """Sum of the row-parallel partial outputs over the TP ranks: the one-shot peer-memory kernel for decode-sized
@@ -342,13 +403,15 @@ class LlamaRuntime:
             out = torch.cat([a * cs - b * sn, a * sn + b * cs], -1)
         return out.to(t.dtype)
 
-    def forward_tokens(self, tokens: torch.Tensor, pos: torch.Tensor, seq: torch.Tensor, cache: KVCache,
+    def forward_tokens(self, tokens: torch.Tensor, pos: torch.Tensor, seq: torch.Tensor, cache: Union[KVCache, PagedKVCache],
                        last_only: Optional[torch.Tensor] = None, max_kv: Optional[int] = None,
                        prefill_bt: Optional[Tuple[int, int]] = None) -> torch.Tensor:
         """``tokens / pos / seq``: ``[n_tok]`` (token id, position in its sequence, sequence index).  The new
         keys/values are appended to ``cache`` and every token attends to positions ``0 .. pos`` of its own
-        sequence.  Returns fp32 logits ``[n_tok or len(last_only), vocab]``."""
+        sequence.  Returns fp32 logits ``[n_tok or len(last_only), vocab]``.  A paged cache must hold pages for the
+        positions (``PagedKVCache.reserve``; ``prefill`` and ``decode_step`` see to it)."""
         cfg = self.cfg
+        paged = isinstance(cache, PagedKVCache)
         C = _native.load(required=True) if self.device.type == "cuda" else None
         n = tokens.shape[0]
         H, Hkv, D = self.h_local, self.hkv_local, cfg.head_dim
@@ -371,7 +434,7 @@ class LlamaRuntime:
         for li, L in enumerate(self.layers):
             rope_done = False
             if fuse:
-                if (cfg.rope_interleaved and QuantLinear.ROPE_FUSED and L.qkv_bias is None and L.wqkv.in_features % 64 == 0
+                if (not paged and cfg.rope_interleaved and QuantLinear.ROPE_FUSED and L.qkv_bias is None and L.wqkv.in_features % 64 == 0
                         and (H + 2 * Hkv) * D % 4 == 0 and not cfg.rope_scaling):
                     # rotary embedding and the cache append ride in the projection's epilogue
                     qkv = L.wqkv.fused(x, norm_w=L.attn_norm, eps=cfg.rms_eps,
@@ -389,7 +452,18 @@ class LlamaRuntime:
             q = qkv[:, : H * D].view(n, H, D)
             k = qkv[:, H * D: (H + Hkv) * D].view(n, Hkv, D)
             v = qkv[:, (H + Hkv) * D:].view(n, Hkv, D)
-            if C is not None:
+            if paged:
+                # rotation (scaled frequencies included) and append in one kernel; the new tokens' own projections take the results
+                paged_append(q, k, v, cache.k[li], cache.v[li], cache.block_table, pos32, seq32, self._inv_freq(D, self.device),
+                             interleaved=cfg.rope_interleaved, q_out=q, k_out=k if flash_bt is not None else None)
+                if flash_bt is None:
+                    att = paged_attention(q, cache.k[li], cache.v[li], cache.block_table, kv_len, seq32, scale=scale)
+                else:
+                    att = torch.empty((n, H, D), dtype=q.dtype, device=q.device)
+                    Bp, Tp = flash_bt
+                    C.attn_fwd(q.unflatten(0, (Bp, Tp)), k.unflatten(0, (Bp, Tp)), v.unflatten(0, (Bp, Tp)), att.view(Bp, Tp, H, D), flash_lse,
+                               True, scale)
+            elif C is not None:
                 if cfg.rope_scaling:
                     # scaled frequencies: the rotation kernels derive theta^(-2i/D) themselves, so these checkpoints
                     # rotate with the frequency table in tensor ops and append to the cache by index
@@ -467,6 +541,9 @@ class LlamaRuntime:
         """``prompts [B, T]`` (equal lengths) -> logits of the last position ``[B, vocab]``."""
         B, T = prompts.shape
         dev = self.device
+        if isinstance(cache, PagedKVCache):
+            for b in range(B):
+                cache.reserve(b, T)
         tokens = prompts.reshape(-1).to(dev)
         pos = torch.arange(T, device=dev).repeat(B)
         seq = torch.arange(B, device=dev).repeat_interleave(T)
@@ -480,6 +557,9 @@ class LlamaRuntime:
         """One new token per sequence: ``tokens [B]`` -> logits ``[B, vocab]``."""
         B = tokens.shape[0]
         dev = self.device
+        if isinstance(cache, PagedKVCache):
+            for b in range(B):
+                cache.reserve(b, cache.lengths[b] + 1)
         pos = torch.tensor(cache.lengths, device=dev)
         seq = torch.arange(B, device=dev)
         logits = self.forward_tokens(tokens.to(dev), pos, seq, cache, max_kv=max(cache.lengths) + 1)
@@ -488,13 +568,23 @@ class LlamaRuntime:
 
     # ----------------------------------------------------------- CUDA-graph decode
     @torch.no_grad()
-    def capture_decode_graph(self, cache: KVCache, batch: int) -> "_DecodeGraph":
-        """Captures one greedy decode step (all layers, lm_head, argmax, position increment) into a CUDA
+    def capture_decode_graph(self, cache: Union[KVCache, PagedKVCache], batch: int, sampling: Optional[SamplingConfig] = None,
+                             uniform: Optional[torch.Tensor] = None) -> "_DecodeGraph":
+        """Captures one decode step (all layers, lm_head, argmax, position increment) into a CUDA
         graph whose inputs live on the device: a step is then one graph launch, and the ~10 launches per
         layer no longer pay host latency.  Positions and the current tokens are device tensors that the graph
-        itself advances, so replaying it N times generates N tokens without any host round trip."""
+        itself advances, so replaying it N times generates N tokens without any host round trip.  With ``sampling``
+        step ``i`` draws its tokens by row ``i`` of ``uniform [steps, batch]`` instead of taking the most likely ones.  The pages of a
+        paged cache have to be reserved before."""
         dev = self.device
         g = _DecodeGraph()
+        if sampling is not None:
+            sampling.validate()
+            if sampling.repetition_penalty != 1.0:
+                raise ValueError("a captured decode step keeps no history: repetition_penalty must be 1")
+            if uniform is None or uniform.dim() != 2 or uniform.shape[1] != batch:
+                raise ValueError("sampling needs random numbers, uniform [steps, batch]")
+            g.uniform = uniform.to(dev)
         g.tok = torch.zeros(batch, dtype=torch.long, device=dev)
         g.pos = torch.zeros(batch, dtype=torch.int32, device=dev)
         g.seq = torch.arange(batch, dtype=torch.int32, device=dev)
@@ -503,7 +593,11 @@ class LlamaRuntime:
 
         def body():
             logits = self.forward_tokens(g.tok, g.pos, g.seq, cache, max_kv=cache.max_len)
-            nxt = logits.argmax(-1)
+            if sampling is None:
+                nxt = logits.argmax(-1)
+            else:
+                nxt = sample_tokens(logits, g.uniform.index_select(0, g.step)[0], temperature=sampling.temperature, top_k=sampling.top_k,
+                                    top_p=sampling.top_p, min_p=sampling.min_p)
             g.out.scatter_(1, g.step.view(1, 1).expand(batch, 1), nxt.view(batch, 1))
             g.tok.copy_(nxt)
             g.pos.add_(1)
@@ -522,18 +616,35 @@ class LlamaRuntime:
         return g
 
     @torch.no_grad()
-    def generate_graph(self, prompts: torch.Tensor, max_new_tokens: int, cache: Optional[KVCache] = None
+    def generate_graph(self, prompts: torch.Tensor, max_new_tokens: int, cache: Optional[Union[KVCache, PagedKVCache]] = None,
+                       sampling: Optional[SamplingConfig] = None, uniform: Optional[torch.Tensor] = None
                        ) -> Tuple[torch.Tensor, Dict[str, float]]:
         """Greedy generation with the decode loop replayed from a CUDA graph (single process or TP ranks that
-        all call it together).  Same outputs as ``generate`` without a sampler."""
+        all call it together).  Same outputs as ``generate`` without a sampler.  With ``sampling`` the tokens are drawn on the
+        device by ``uniform [max_new_tokens, B]`` (row 0: the token after the prompt), by default numbers from ``sampling.seed``."""
         B, T = prompts.shape
         cache = cache or self.new_cache(B, T + max_new_tokens)
         dev = self.device
-        g = self.capture_decode_graph(cache, B)           # the warm-up/capture writes only at position 0.. (reset below)
+        if isinstance(cache, PagedKVCache):
+            for b in range(B):
+                cache.reserve(b, T + max_new_tokens)
+        if sampling is not None:
+            if uniform is None:
+                gen = torch.Generator().manual_seed(sampling.seed) if sampling.seed is not None else None
+                uniform = torch.rand(max_new_tokens, B, generator=gen)
+            if uniform.shape != (max_new_tokens, B):
+                raise ValueError(f"uniform must be [{max_new_tokens}, {B}], got {list(uniform.shape)}")
+            uniform = uniform.to(dev)
+        # the warm-up/capture writes only at position 0.. (reset below)
+        g = self.capture_decode_graph(cache, B, sampling, uniform[1:] if uniform is not None and max_new_tokens > 1 else uniform)
         torch.cuda.synchronize(dev)
         t0 = time.perf_counter()
         logits = self.prefill(prompts, cache)
-        nxt = logits.argmax(-1)
+        if sampling is None:
+            nxt = logits.argmax(-1)
+        else:
+            nxt = sample_tokens(logits, uniform[0].contiguous(), temperature=sampling.temperature, top_k=sampling.top_k, top_p=sampling.top_p,
+                                min_p=sampling.min_p)
         g.tok.copy_(nxt)
         g.pos.fill_(T)
         g.step.zero_()

@@ -1,4 +1,5 @@
-"""Token sampling: temperature, top-k, top-p (nucleus), repetition penalty, multinomial draw
+"""Token sampling: temperature, top-k, top-p (nucleus), min-p, repetition penalty, multinomial draw, and a draw from given
+random numbers in one kernel (``Sampler.draw``)
 (example-cli/src/model/sampling.rs:8-300; the reference's ``sample_token`` is a placeholder returning
 ``vocab/2`` and its repetition penalty is a TODO)."""
 from __future__ import annotations
@@ -16,6 +17,7 @@ class SamplingConfig:
     top_p: float = 1.0        # 1.0 = disabled
     repetition_penalty: float = 1.0
     seed: Optional[int] = None
+    min_p: float = 0.0        # 0.0 = disabled
 
     def validate(self) -> None:
         if self.temperature < 0:
@@ -26,6 +28,8 @@ class SamplingConfig:
             raise ValueError("top_p must be in (0, 1]")
         if self.repetition_penalty <= 0:
             raise ValueError("repetition_penalty must be > 0")
+        if not 0.0 <= self.min_p <= 1.0:
+            raise ValueError("min_p must be in [0, 1]")
 
     @staticmethod
     def greedy() -> "SamplingConfig":
@@ -65,6 +69,14 @@ def apply_top_p_to_probs(probs: torch.Tensor, top_p: float) -> torch.Tensor:
     return p / p.sum(-1, keepdim=True)
 
 
+def apply_min_p_to_probs(probs: torch.Tensor, min_p: float) -> torch.Tensor:
+    """Drop tokens of less than ``min_p`` times the largest probability."""
+    if min_p <= 0.0:
+        return probs
+    p = torch.where(probs < min_p * probs.amax(-1, keepdim=True), torch.zeros_like(probs), probs)
+    return p / p.sum(-1, keepdim=True)
+
+
 def multinomial_sample(probs: torch.Tensor, generator: Optional[torch.Generator] = None) -> torch.Tensor:
     return torch.multinomial(probs, 1, generator=generator).squeeze(-1)
 
@@ -89,9 +101,21 @@ class Sampler:
             tok = logits.argmax(-1)
         else:
             probs = softmax(logits / c.temperature)
-            probs = apply_top_p_to_probs(apply_top_k_to_probs(probs, c.top_k), c.top_p)
+            probs = apply_min_p_to_probs(apply_top_p_to_probs(apply_top_k_to_probs(probs, c.top_k), c.top_p), c.min_p)
             gen = self._gen if (self._gen is not None and self._gen.device == probs.device) else None
             tok = multinomial_sample(probs, gen)
+        t = tok.view(-1, 1)
+        self.history = t if self.history is None else torch.cat([self.history, t], 1)
+        return tok
+
+    def draw(self, logits: torch.Tensor, uniform: torch.Tensor) -> torch.Tensor:
+        """``logits [B, V]`` and numbers ``uniform [B]`` in ``[0, 1)`` -> tokens ``[B]`` by the same settings: one kernel on CUDA
+        (``ops.sampling.sample_tokens``), a function of its arguments and the history alone."""
+        from ..ops.sampling import sample_tokens
+        c = self.config
+        if self.history is not None and c.repetition_penalty != 1.0:
+            logits = apply_repetition_penalty(logits.float(), self.history, c.repetition_penalty)
+        tok = sample_tokens(logits, uniform, temperature=c.temperature, top_k=c.top_k, top_p=c.top_p, min_p=c.min_p)
         t = tok.view(-1, 1)
         self.history = t if self.history is None else torch.cat([self.history, t], 1)
         return tok
