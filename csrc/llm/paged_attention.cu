@@ -39,6 +39,9 @@ constexpr int PA_WARPS = 4;
 constexpr int PA_TILE = 16;                    // keys of one warp step
 constexpr int PA_UNIT = PA_WARPS * PA_TILE;    // keys of one CTA step
 constexpr float PA_LOG2E = 1.4426950408889634f;
+// Units of a share at least: 4 sequences of 4000 keys on one head 37 us with one, 22 with two, 22 with four; 77 keys of 32 heads
+// 9, 6.7, 9.5 us; 2048 keys of 8 heads 11.6, 11.2, 12.4.
+constexpr int PA_MIN_SHARE = 2;
 // The running maximum is moved only when a score exceeds it by PA_SLACK (base 2), and then set PA_ROOM below the score: weights
 // reach 2^14 at most, which fits fp16, and small ones keep more of its digits than with the maximum itself.
 constexpr float PA_SLACK = 14.f, PA_ROOM = 4.f;
@@ -53,7 +56,8 @@ template <int DP, int NH> struct Cfg {         // DP: head size rounded up, NH: 
   static constexpr int OFF_Q = STAGES * PA_WARPS * STAGE;
   static constexpr int OFF_ACC = OFF_Q + (STAGES + 1) * QBUF;
   static constexpr int OFF_ML = OFF_ACC + 2 * HEADS * ACC_LD * 4;
-  static constexpr int OFF_TOK = OFF_ML + (2 * PA_WARPS + 3) * HEADS * 4;
+  static constexpr int OFF_FAC = OFF_ML + (2 * PA_WARPS + 3) * HEADS * 4;
+  static constexpr int OFF_TOK = OFF_FAC + 32 * HEADS * 4;
   static constexpr int SMEM = OFF_TOK + PAGED_ATTN_CHUNK * 20 + 8;
   static constexpr int PART = HEADS * (DP + 2);                // floats of a part: rows, maxima, sums
   static constexpr bool Q_IN_REGS = DP * NH <= 256;
@@ -170,11 +174,11 @@ paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, bool 
   }
   if (tid == 0) tk.first[n] = U;
   __syncthreads();
-  const int P = (int)min((long long)gridDim.x, U);  // every share holds a unit at least
+  const int P = (int)min((long long)gridDim.x, max(1ll, U / PA_MIN_SHARE));
   for (int t = blockIdx.x; t < n; t += gridDim.x)
     if (tk.len[t] == 0)
       for (int i = tid; i < a.H * c.D; i += blockDim.x) put((T*)a.out + (t0 + t) * a.o_st + (i / c.D) * a.o_sh + i % c.D, 0.f);
-  if (blockIdx.x >= P) return;
+  if (U == 0 || blockIdx.x >= P) return;
   const long long ub = U * blockIdx.x / P, ue = U * (blockIdx.x + 1) / P;
 
   auto enter = [&](Walk& w, long long rem) {  // rem: units from the token's first
@@ -294,6 +298,7 @@ paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, bool 
   float* sm_sum = sm_top + HEADS;
   float* sm_inv = sm_sum + HEADS;
   static_assert(2 * HEADS * C::ACC_LD >= PA_WARPS * 32 * 4, "the join's sums fit the merge buffer");
+  float* sm_fac = reinterpret_cast<float*>(smem + C::OFF_FAC);  // [32][HEADS] factors of the parts that are joined
   float4* join_buf = reinterpret_cast<float4*>(smem + C::OFF_ACC);
   // ldmatrix lanes: A fragments of K (rows are keys) and, transposed, of V; B fragments of Q
   const uint32_t k_lane = sbase + warp * C::STAGE + ((lane & 7) + ((lane >> 3) & 1) * 8) * C::ROW + (lane >> 4) * 16;
@@ -515,53 +520,78 @@ paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, bool 
         __threadfence();
         const int parts = c1 - c0 + 1;
         auto from = [&](int k) { return part + ((long long)(c0 + k) * 2 + (k == 0 ? 1 : 0)) * C::PART; };
-        for (int r = warp; r < rows; r += PA_WARPS) {
-          float big = -CUDART_INF_F, x = 0.f;
-          for (int k = lane; k < parts; k += 32) big = fmaxf(big, __ldcg(from(k) + HEADS * DP + r));
+        constexpr int RW = HEADS / PA_WARPS;  // rows of a warp: warp + 4 i
+        float big[RW], sum[RW], m0[RW], l0[RW];
 #pragma unroll
-          for (int d = 16; d > 0; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
-          for (int k = lane; k < parts; k += 32) x = fmaf(__ldcg(from(k) + HEADS * (DP + 1) + r), factor(__ldcg(from(k) + HEADS * DP + r), big), x);
-#pragma unroll
-          for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-          if (lane == 0) {
-            sm_top[r] = big;
-            sm_inv[r] = x == 0.f ? 0.f : 1.f / x;
-          }
+        for (int i = 0; i < RW; ++i) {  // the lane's first part, all rows at once
+          const int r = warp + PA_WARPS * i;
+          const bool in = lane < parts && r < rows;
+          m0[i] = in ? __ldcg(from(lane) + HEADS * DP + r) : -CUDART_INF_F;
+          l0[i] = in ? __ldcg(from(lane) + HEADS * (DP + 1) + r) : 0.f;
         }
-        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+          const int r = warp + PA_WARPS * i;
+          big[i] = m0[i];
+          if (r < rows)
+            for (int k = lane + 32; k < parts; k += 32) big[i] = fmaxf(big[i], __ldcg(from(k) + HEADS * DP + r));
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1) big[i] = fmaxf(big[i], __shfl_xor_sync(0xffffffffu, big[i], d));
+          sum[i] = l0[i] * factor(m0[i], big[i]);
+          if (r < rows)
+            for (int k = lane + 32; k < parts; k += 32)
+              sum[i] = fmaf(__ldcg(from(k) + HEADS * (DP + 1) + r), factor(__ldcg(from(k) + HEADS * DP + r), big[i]), sum[i]);
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], d);
+          if (lane == 0 && r < rows) sm_inv[r] = sum[i] == 0.f ? 0.f : 1.f / sum[i];
+        }
         int split = 1;  // threads that share four values
         while (quads * split * 2 <= PA_WARPS * 32 && split * 2 <= parts) split *= 2;
-        const int group = tid / quads;
-        const int step_q = split > 1 ? quads : PA_WARPS * 32;
-        for (int i = split > 1 ? tid % quads : tid; i < quads; i += step_q) {
-          const int r = i / D4, d = i % D4 * 4;
-          float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (d < c.D && group < split || split == 1) {
-            const float big = sm_top[r];
+        constexpr int QT = (HEADS * D4 + PA_WARPS * 32 - 1) / (PA_WARPS * 32);  // fours of a thread, where there is one for each
+        float4 z[QT];
+#pragma unroll
+        for (int q = 0; q < QT; ++q) z[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int group = split > 1 ? tid / quads : 0;
+        for (int k0 = 0; k0 < parts; k0 += 32) {
+#pragma unroll
+          for (int i = 0; i < RW; ++i) {
+            const int r = warp + PA_WARPS * i, k = k0 + lane;
+            const float m = k0 == 0 ? m0[i] : k < parts && r < rows ? __ldcg(from(k) + HEADS * DP + r) : -CUDART_INF_F;
+            sm_fac[lane * HEADS + r] = factor(m, big[i]);
+          }
+          __syncthreads();
+          const int end_k = min(parts, k0 + 32);
+#pragma unroll
+          for (int q = 0; q < QT; ++q) {
+            const int i = split > 1 ? tid % quads : tid + q * PA_WARPS * 32;
+            const int r = i / D4, d = i % D4 * 4;
+            if (i < quads && group < split && d < c.D && (q == 0 || split == 1)) {
 #pragma unroll 8
-            for (int k = split > 1 ? group : 0; k < parts; k += split) {
-              const float* p = from(k);
-              const float f = factor(__ldcg(p + HEADS * DP + r), big);
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(p + r * DP + d));
-              z = make_float4(fmaf(x.x, f, z.x), fmaf(x.y, f, z.y), fmaf(x.z, f, z.z), fmaf(x.w, f, z.w));
+              for (int k = k0 + group; k < end_k; k += split) {
+                const float f = sm_fac[(k - k0) * HEADS + r];
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(from(k) + r * DP + d));
+                z[q] = make_float4(fmaf(x.x, f, z[q].x), fmaf(x.y, f, z[q].y), fmaf(x.z, f, z[q].z), fmaf(x.w, f, z[q].w));
+              }
             }
           }
-          if (split == 1) {
-            if (d < c.D) store(r, d, z, sm_inv[r]);
-          } else if (group < split) {
-            join_buf[group * quads + i] = z;
-          }
-          if (split > 1) break;
+          __syncthreads();
         }
-        if (split > 1) {
+        if (split == 1) {
+#pragma unroll
+          for (int q = 0; q < QT; ++q) {
+            const int i = tid + q * PA_WARPS * 32, d = i % D4 * 4;
+            if (i < quads && d < c.D) store(i / D4, d, z[q], sm_inv[i / D4]);
+          }
+        } else {
+          if (group < split) join_buf[tid] = z[0];
           __syncthreads();
           if (tid < quads && tid % D4 * 4 < c.D) {
-            float4 z = join_buf[tid];
+            float4 x = join_buf[tid];
             for (int g = 1; g < split; ++g) {
-              const float4 x = join_buf[g * quads + tid];
-              z = make_float4(z.x + x.x, z.y + x.y, z.z + x.z, z.w + x.w);
+              const float4 y = join_buf[g * quads + tid];
+              x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
             }
-            store(tid / D4, tid % D4 * 4, z, sm_inv[tid / D4]);
+            store(tid / D4, tid % D4 * 4, x, sm_inv[tid / D4]);
           }
         }
         if (tid == 0) counters[c0] = 0;  // for the next launch that uses this workspace
