@@ -137,7 +137,8 @@ Tensor attention_workspace(const Tensor& like, int64_t bytes) {
     C10_CUDA_CHECK(cudaMemsetAsync(t.data_ptr(), 0, rt::PAGED_ATTN_COUNTER_BYTES, stream));
     return t;
   };
-  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return fresh();
+  // (the per-thread default stream is one handle for many streams)
+  if (stream == cudaStreamPerThread || c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return fresh();
   static std::mutex mu;
   static auto* kept = new std::map<std::pair<int, cudaStream_t>, Tensor>();  // outlives the allocator's own shutdown
   std::lock_guard<std::mutex> lock(mu);
@@ -160,7 +161,8 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& 
   TORCH_CHECK(a.cache.s_page % 8 == 0 && a.cache.s_head % 8 == 0 && a.cache.s_row % 8 == 0 && reinterpret_cast<uintptr_t>(a.cache.k) % 16 == 0 &&
                   reinterpret_cast<uintptr_t>(a.cache.v) % 16 == 0,
               op, ": the rows of the pages must start on 16-byte boundaries");
-  TORCH_CHECK(std::isfinite(scale) && std::isfinite(softcap) && softcap >= 0, op, ": scale must be finite, softcap finite and not negative");
+  TORCH_CHECK(std::isfinite(scale) && std::abs(scale) <= 1e30, op, ": scale must be finite");
+  TORCH_CHECK(softcap == 0 || (softcap >= 1e-6 && softcap <= 1e30), op, ": softcap must be 0 (none) or from 1e-6 to 1e30");
   TORCH_CHECK(window >= 0, op, ": window must not be negative");
   TORCH_CHECK(n < (1ll << 31), op, ": too many tokens for one call");
   c10::cuda::CUDAGuard guard(q_in.device());

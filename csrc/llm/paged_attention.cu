@@ -92,6 +92,15 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float 
 __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half(v); }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
 
+// 1 - 2 / (exp(2x) + 1) is off by 2^-22 of one; near zero, where that would be much of the result, four terms of the series
+// x - x^3 / 3 + 2 x^5 / 15 - 17 x^7 / 315 (the next is below 2e-9 of x for |x| < 1/8).
+__device__ __forceinline__ float tanh_of(float x) {
+  const float q = x * x;
+  const float near = x * fmaf(q, fmaf(q, fmaf(q, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
+  const float far = 1.f - 2.f / (ex2_approx(x * (2.f * PA_LOG2E)) + 1.f);
+  return q < 1.f / 64.f ? near : far;
+}
+
 // What a chunk of tokens looks like to the schedule, in shared memory.
 struct Tokens {
   long long* first;  // units of the tokens before this one, all heads
@@ -289,7 +298,7 @@ paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, bool 
   for (int i = 0; i < S; ++i) issue(i);
 
   // ---- items
-  const float scale2 = a.softcap > 0.f ? a.scale / a.softcap * (2.f * PA_LOG2E) : a.scale * PA_LOG2E;
+  const float scale2 = a.softcap > 0.f ? a.scale / a.softcap : a.scale * PA_LOG2E;
   const float cap2 = a.softcap * PA_LOG2E;
   float* acc_buf = reinterpret_cast<float*>(smem + C::OFF_ACC);
   float* sm_m = reinterpret_cast<float*>(smem + C::OFF_ML);
@@ -363,7 +372,7 @@ paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, bool 
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float x = (s[h][0][e] + s[h][1][e]) * scale2;
-            if (a.softcap > 0.f) x = cap2 - 2.f * cap2 / (ex2_approx(x) + 1.f);  // tanh(y) = 1 - 2 / (exp(2y) + 1), error absolute as a score's may be
+            if (a.softcap > 0.f) x = cap2 * tanh_of(x);
             if (!all && !(mask >> ((lane >> 2) + (e < 2 ? 0 : 8)) & 1)) x = -CUDART_INF_F;
             grow |= x > m[h][e & 1] + PA_SLACK;
             s[h][0][e] = x;

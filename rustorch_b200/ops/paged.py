@@ -48,7 +48,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     ``q [n, H, D]`` (``H`` a multiple of the cache's heads, ``D`` a multiple of 8 up to 256), ``kv_len``, ``seq``: int32 ``[n]``.
     ``window > 0`` keeps the last ``window`` of these positions, ``softcap > 0`` applies
-    ``f(x) = softcap tanh(x / softcap)``; ``scale`` defaults to ``1 / sqrt(D)``.  A token that sees no position gets zeros.
+    ``f(x) = softcap tanh(x / softcap)`` (1e-6 to 1e30); ``scale`` defaults to ``1 / sqrt(D)``.  A token that sees no position gets zeros.
     What the cache holds beyond the visible positions (NaN included) does not matter.  Inference only: no gradients.
     """
     if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
@@ -118,8 +118,8 @@ def _attention_cpu(q, k_pages, v_pages, block_table, kv_len, seq, scale, window,
     hkv, page, D = k_pages.shape[1:]
     if q.dim() != 3 or q.shape[2] != D or q.shape[1] == 0 or q.shape[1] % hkv:
         raise RuntimeError(f"{op}: q must be [n_tok, heads, head_dim] with a multiple of {hkv} heads")
-    if not (math.isfinite(scale) and math.isfinite(softcap)) or softcap < 0 or window < 0:
-        raise RuntimeError(f"{op}: scale must be finite, softcap finite and not negative, window not negative")
+    if not abs(scale) <= 1e30 or not (softcap == 0 or 1e-6 <= softcap <= 1e30) or window < 0:
+        raise RuntimeError(f"{op}: scale must be finite, softcap 0 (none) or from 1e-6 to 1e30, window not negative")
     res = torch.zeros(n, q.shape[1], D, dtype=q.dtype)
     for t in range(n):
         s, length = t if seq is None else int(seq[t]), int(kv_len[t])

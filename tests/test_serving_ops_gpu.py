@@ -160,6 +160,27 @@ def test_attention_extreme_scores():
     assert ((out[0].double() - want).abs() <= (half_step(torch.float16) + 600 * 2.0 ** -24) * 4 + half_step(torch.float16) * want.abs()).all()
 
 
+@pytest.mark.parametrize("softcap", [1e5, 1e30])
+def test_attention_cap_far_above_the_scores(softcap):
+    """cap tanh(x / cap) - x is x^3 / (3 cap^2), nothing here: the tolerance is that of uncapped scores, whose ``(D + 4) 2^-24`` of
+    the products' sizes covers the eight roundings of the capped form."""
+    _, attention, _ = _ops()
+    g = torch.Generator().manual_seed(8)
+    kp, vp, table = paged_cache([700], 2, 16, 64, torch.float16, "cuda", g)
+    q = torch.randn(1, 4, 64, generator=g).half().cuda()
+    want, tol = attend(q, kp, vp, table, [700], None, 0.5)
+    _check(attention(q, kp, vp, table, _i32([700]), scale=0.5, softcap=softcap), want, tol)
+
+
+def test_attention_writes_over_its_queries():
+    _, attention, _ = _ops()
+    g = torch.Generator().manual_seed(9)
+    kp, vp, table = paged_cache([3000, 5, 0], 2, 16, 128, torch.bfloat16, "cuda", g)
+    q = torch.randn(3, 40, 128, generator=g).bfloat16().cuda()
+    want = attention(q, kp, vp, table, _i32([3000, 5, 0]))
+    assert attention(q, kp, vp, table, _i32([3000, 5, 0]), out=q) is q and torch.equal(q, want)
+
+
 # ------------------------------------------------------------------------------------------------------------ sampling
 def _logits(rows, vocab, dtype, gen):
     x = torch.randn(rows, vocab, generator=gen) * 2
@@ -204,6 +225,27 @@ def test_sampling_rows_with_their_own_settings(rows, vocab, dtype):
     got = sample(wide.cuda()[:, 1:vocab + 1], u.cuda(), temperature=t.cuda(), top_k=k.cuda(), top_p=p.cuda(), min_p=m.cuda())
     want = [draw_token(x[r], float(u[r]), float(t[r]), int(k[r]), max(1e-300, float(p[r])), float(m[r])) for r in range(rows)]
     assert got.tolist() == want
+
+
+@pytest.mark.parametrize("temperature", [1e-45, 1e-6, 1e30, 1e300])
+@pytest.mark.parametrize("top_k,top_p,min_p", [(0, 1.0, 0.0), (7, 1.0, 0.0), (0, 0.7, 0.0), (900, 0.5, 0.3)])
+def test_sampling_extreme_temperatures(temperature, top_k, top_p, min_p):
+    _, _, sample = _ops()
+    g = torch.Generator().manual_seed(4)
+    x, u = _logits(9, 2000, torch.float32, g), torch.rand(9, generator=g)
+    want = [draw_token(x[r], float(u[r]), temperature, top_k, top_p, min_p) for r in range(9)]
+    assert sample(x.cuda(), u.cuda(), temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p).tolist() == want
+
+
+def test_sampling_many_near_ties():
+    """Logits that lie within a few steps of the finest histogram, and an all-but-equal row over its list's length."""
+    _, _, sample = _ops()
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(6, 30000, generator=g) * 1e-4 + torch.tensor([0.0, 1.0, -3.0, 100.0, 1e-3, 7.0])[:, None]
+    u = torch.rand(6, generator=g)
+    for kw in (dict(top_k=15000), dict(top_p=0.5), dict(top_k=20000, top_p=0.3), dict(min_p=0.9999)):
+        want = [draw_token(x[r], float(u[r]), 1.0, kw.get("top_k", 0), kw.get("top_p", 1.0), kw.get("min_p", 0.0)) for r in range(6)]
+        assert sample(x.cuda(), u.cuda(), **kw).tolist() == want, kw
 
 
 def test_sampling_frequencies():
@@ -371,7 +413,7 @@ def test_refusals_on_the_device():
     for kw in (dict(q=q.float()), dict(q=q.bfloat16()), dict(q=q[:, :3]), dict(q=q[0]), dict(q=q.cpu()), dict(kv_len=i1.long()), dict(kv_len=i1.cpu()),
                dict(seq=_i32([0, 0])), dict(block_table=table.long()), dict(block_table=table[0]), dict(k_pages=odd, v_pages=odd),
                dict(v_pages=kp.transpose(1, 2).contiguous().transpose(1, 2)), dict(k_pages=kp[:1]), dict(window=-1), dict(softcap=-1.0),
-               dict(softcap=float("inf")), dict(scale=float("nan")), dict(out=torch.zeros(1, 4, 64, device="cuda")), dict(out=k),
+               dict(softcap=float("inf")), dict(softcap=1e-9), dict(scale=float("nan")), dict(scale=1e31), dict(out=torch.zeros(1, 4, 64, device="cuda")), dict(out=k),
                dict(out=q[:, :1].expand(-1, 4, -1)), dict(q=torch.zeros(1, 4, 60, dtype=torch.half, device="cuda")),
                dict(q=torch.zeros(1, 4, 320, dtype=torch.half, device="cuda"), k_pages=torch.zeros(2, 2, 4, 320, dtype=torch.half, device="cuda"),
                     v_pages=torch.zeros(2, 2, 4, 320, dtype=torch.half, device="cuda"))):
