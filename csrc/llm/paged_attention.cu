@@ -13,12 +13,14 @@
 // arrives last at its counter joins them in share order, so the result does not depend on timing.
 //
 // Inside a CTA each of four warps owns 16 keys of a unit and its own ring of stages, without block barriers between
-// units; the ring runs on across items.  Rows are copied by cp.async with their 16-byte pieces on neighbouring lanes: over 131072
-// keys (32 heads on 8, D = 128) 92 us and 6.9 TB/s from one length to the next.  The same rows in 64-byte steps on four lanes
-// took 122 us, as one bulk copy each 124 us (the copy engine takes one every 8 cycles, and a tile is 32 of them).  The products are m16n8k16 with the cache as the 16 rows and eight query
-// heads as the columns: S^T = K Q^T (16 keys), O^T += V^T P^T (16 of D).  Decode has 1 to 16 query heads a kv head, a
-// corner of a 128-row tcgen05 tile; here the tensor time is a fraction of the load time.  Rows that are not visible are not
-// copied: a tile that has some masks their scores, and their values too, which may be left-over NaN.
+// units; the ring runs on across items.  Rows are copied by cp.async with their 16-byte pieces on neighbouring lanes: 131072 keys
+// (32 heads on 8, D = 128) take 94 us, 6.9 TB/s from one length to the next.  The same rows in 64-byte steps on four lanes
+// took 122 us, as one bulk copy each 124 us (the copy engine takes one every 8 cycles, and a tile is 32 of them); keys and
+// values as two groups, refilled one after the other, 118 us; a window of 32 block-table entries in registers 100 us.
+// The products are m16n8k16 with the cache as the 16 rows and eight query heads as the columns: S^T = K Q^T (16 keys),
+// O^T += V^T P^T (16 of D).  Decode has 1 to 16 query heads a kv head, a corner of a 128-row tcgen05 tile; here the tensor
+// time is a fraction of the load time.  Weights enter the second product rounded to the values' type, as the result is.
+// Rows that are not visible are not copied: a tile that has some masks their scores, and their values too, which may be left-over NaN.
 // Maximum, sum and output are kept in 32 bits.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
