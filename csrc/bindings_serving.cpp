@@ -214,7 +214,8 @@ Tensor sample_tokens(const Tensor& logits, const Tensor& uniform, double tempera
   a.top_p_rows = rows_f32(top_p_rows, "top_p");
   a.min_p_rows = rows_f32(min_p_rows, "min_p");
   if (given(top_k_rows)) a.top_k_rows = check_index(*top_k_rows, logits, B, op, "top_k per row");
-  TORCH_CHECK(temperature >= 0 && std::isfinite(temperature), op, ": temperature must be finite and not negative");
+  // settings are 32-bit numbers, whether they come one a row or one for all
+  TORCH_CHECK(temperature >= 0 && std::isfinite(float(temperature)), op, ": temperature must be a finite 32-bit number and not negative");
   TORCH_CHECK(top_k >= 0, op, ": top_k must not be negative");
   TORCH_CHECK(top_p > 0 && top_p <= 1, op, ": top_p must be in (0, 1]");
   TORCH_CHECK(min_p >= 0 && min_p <= 1, op, ": min_p must be in [0, 1]");
@@ -226,9 +227,9 @@ Tensor sample_tokens(const Tensor& logits, const Tensor& uniform, double tempera
   a.vocab = int(V);
   a.uniform = uniform.data_ptr();
   a.uniform_f64 = uniform.scalar_type() == at::kDouble;
-  a.temperature = temperature;
-  a.top_p = top_p;
-  a.min_p = min_p;
+  a.temperature = float(temperature);
+  a.top_p = float(top_p);
+  a.min_p = float(min_p);
   a.top_k = int(std::min<int64_t>(top_k, V));
   a.out = reinterpret_cast<long long*>(out.data_ptr<int64_t>());
   rt::sample_tokens(a, stream_of(logits));

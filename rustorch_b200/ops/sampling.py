@@ -24,8 +24,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: S
     least ``min_p`` times the largest weight.  The token is the first one, in the vocabulary's order, at which the running sum
     of the kept weights exceeds ``uniform`` times their sum; it follows from the inputs alone, whatever the batch.
 
-    Each setting is a number or a tensor with one value a row (int32 for ``top_k``, fp32 for the others).  Temperature 0 takes the
-    most likely token (lowest index of equals).  Logits of minus infinity and NaN are never drawn; a row that has no
+    Each setting is a number or a tensor with one value a row (int32 for ``top_k``, fp32 for the others; numbers are rounded to
+    fp32, so both forms draw alike).  Temperature 0 takes the most likely token (lowest index of equals).  Logits of minus infinity and NaN are never drawn; a row that has no
     other gives -1.  Tokens of less than 1.4e-14 times the largest weight count as impossible.
     """
     scalars, rows = [], []
@@ -49,8 +49,9 @@ def _sample_cpu(logits, uniform, temperature, top_k, top_p, min_p, temperature_r
                             ("top_k", top_k_rows, (torch.int32,)), ("top_p", top_p_rows, (torch.float32,)), ("min_p", min_p_rows, (torch.float32,))):
         if x is not None and (x.dtype not in dtypes or x.shape != (rows,)):
             raise RuntimeError(f"sample_tokens: {name} must be one {' or '.join(map(str, dtypes))} a row")
-    if not (temperature >= 0 and math.isfinite(temperature)) or top_k < 0 or not 0 < top_p <= 1 or not 0 <= min_p <= 1:
+    if not 0 <= temperature <= torch.finfo(torch.float32).max or top_k < 0 or not 0 < top_p <= 1 or not 0 <= min_p <= 1:
         raise RuntimeError("sample_tokens: temperature and top_k must not be negative, top_p in (0, 1], min_p in [0, 1]")
+    temperature, top_p, min_p = torch.tensor([temperature, top_p, min_p], dtype=torch.float32).tolist()
     out = torch.empty(rows, dtype=torch.int64)
     for r in range(rows):
         l = logits[r].double().nan_to_num(nan=-math.inf, posinf=math.inf, neginf=-math.inf)

@@ -63,7 +63,8 @@ def attend(q, k_pages, v_pages, table, kv_len, seq, scale, window=0, softcap=0.0
 
 
 def draw_token(logits, u, temperature, top_k, top_p, min_p):
-    """Token of one row of logits (any dtype) in 64 bits."""
+    """Token of one row of logits (any dtype) in 64 bits, by settings that are 32-bit numbers."""
+    temperature, top_p, min_p = torch.tensor([temperature, top_p, min_p], dtype=torch.float32).tolist()
     l = [float(x) for x in logits.double()]
     l = [-math.inf if x != x else x for x in l]
     best = max(l)

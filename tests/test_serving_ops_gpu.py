@@ -210,6 +210,9 @@ def test_sampling_against_the_definition(dtype, vocab, temperature, top_k, top_p
     want = [draw_token(x[r], float(u[r]), temperature, top_k, top_p, min_p) for r in range(rows)]
     got = sample(x.cuda(), u.cuda(), temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
     assert got.dtype == torch.int64 and got.tolist() == want
+    every = {k: torch.full((rows,), v, dtype=torch.int32 if k == "top_k" else torch.float32, device="cuda")
+             for k, v in dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p).items()}
+    assert torch.equal(sample(x.cuda(), u.cuda(), **every), got)                 # one setting for all, or the same for every row
 
 
 @pytest.mark.parametrize("rows,vocab,dtype", [(1, 128256, torch.float32), (3, 262144, torch.bfloat16), (4, 50257, torch.bfloat16), (200, 1000, torch.float32)])
@@ -227,7 +230,7 @@ def test_sampling_rows_with_their_own_settings(rows, vocab, dtype):
     assert got.tolist() == want
 
 
-@pytest.mark.parametrize("temperature", [1e-45, 1e-6, 1e30, 1e300])
+@pytest.mark.parametrize("temperature", [1e-45, 1e-6, 1e30, 3e38])
 @pytest.mark.parametrize("top_k,top_p,min_p", [(0, 1.0, 0.0), (7, 1.0, 0.0), (0, 0.7, 0.0), (900, 0.5, 0.3)])
 def test_sampling_extreme_temperatures(temperature, top_k, top_p, min_p):
     _, _, sample = _ops()
@@ -429,7 +432,8 @@ def test_refusals_on_the_device():
             append(**{**good, **kw})
     x, u = torch.zeros(2, 9, device="cuda"), torch.zeros(2, device="cuda")
     for kw in (dict(logits=x.double()), dict(logits=x[0]), dict(logits=x.t()), dict(uniform=u.half()), dict(uniform=u[:1]), dict(uniform=u.cpu()),
-               dict(temperature=-1.0), dict(temperature=float("nan")), dict(top_k=-1), dict(top_p=0.0), dict(top_p=1.1), dict(min_p=2.0),
+               dict(temperature=-1.0), dict(temperature=float("nan")), dict(temperature=1e39), dict(top_k=-1), dict(top_p=0.0), dict(top_p=1.1),
+               dict(min_p=2.0),
                dict(temperature=u.double()), dict(top_k=u), dict(top_p=u[:1]), dict(min_p=u.cpu()),
                dict(logits=torch.zeros(2, 262145, device="cuda"))):
         with pytest.raises(RuntimeError):
