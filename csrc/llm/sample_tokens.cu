@@ -16,6 +16,7 @@
 // go on over their keys.  Members of a crossing step are queued by the one pass that compares floats to find them, and only the queue is
 // looked at again.  The draw needs each CTA's kept weight, which its part of the first histogram and the queue give; then only the
 // CTA that holds the target adds by warp, by parts of a warp's stretch, and walks.
+// A top_k whose candidates fit one CTA (384) is finished there, all filters and the draw (1 x 32000, top_k 50, top_p 0.9: 10 us, 21 without).
 // Bound by issue slots where all weights are summed (top_p or no filter): a 64-bit exponential is 18 instructions a logit.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -38,6 +39,7 @@ typedef unsigned long long u64;
 constexpr int ST_THREADS = 384, ST_WARPS = ST_THREADS / 32;  // three CTAs an SM beside 64 KB slices
 constexpr int ST_MAX_CLUSTER = 8;
 constexpr int ST_BINS = ST_THREADS;            // a bin a thread where sums over them are formed
+constexpr int ST_FEW = ST_THREADS;             // candidates that one CTA finishes, a thread each
 constexpr int ST_LIST = 64;                    // members of a step that a warp ranks
 constexpr int ST_QUEUE = 512;                  // members of a step that a CTA keeps at hand
 constexpr int ST_TABLE = 128;                  // 2^(i / 128)
@@ -60,14 +62,16 @@ struct alignas(16) Shared {
   u64 part[2][ST_WARPS];                       // reductions by warp, used in turn
   u64 mass[ST_WARPS], fine_mass[ST_WARPS];     // draw: kept weight above the cut, by warp
   unsigned ties[ST_WARPS], fine_ties[ST_WARPS];  // draw: members at the cut, by warp
-  unsigned lo[2][ST_BINS], hi[2][ST_BINS];     // histograms (the first, and finer ones): counts in lo, weights in both
+  struct {
+    unsigned lo[ST_BINS], hi[ST_BINS];         // counts in lo, weights in both
+  } hist[2];                                   // the first histogram, and finer ones; of the first CTA also the few of a small top_k
   unsigned list[2][ST_LIST];                   // keys of a finer step's members, for top_k and for top_p (the first CTA's)
   float queue[ST_QUEUE];                       // this CTA's members of the crossing step
   int n_list[2], n_queue;
   u64 cta_mass;                                // draw: of the whole CTA
   unsigned cta_ties;
   // what one thread finds for its CTA
-  u64 found_mass;
+  u64 found_mass, found_upto;
   unsigned found_key;
   int found_bin;
 };
@@ -253,6 +257,15 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
   auto steps_to = [](double p) { return fminf(fmaxf(-log2f((float)p) * (float)((ST_BINS - 1) / ST_OCTAVES), 0.f) + 0.01f, ST_BINS - 1.f); };
   const float min_steps = steps_to(min_p);
   const bool by_count = top_k > 0 && top_k < a.vocab, by_mass = top_p < 1.0;
+  auto wanted = [&](u64 total) -> u64 {  // the mass that top_p asks for, a part of the first token at least
+    const double some = ceil((top_p > 0.0 ? top_p : 0.0) * (double)total);
+    return some >= 1.0 ? (some < (double)total ? (u64)some : total) : 1;
+  };
+  auto fraction = [&]() -> u64 {  // the row's number in 2^-64
+    double u = a.uniform_f64 ? ((const double*)a.uniform)[row] : (double)((const float*)a.uniform)[row];
+    u = u > 0.0 ? u : 0.0;
+    return u < 1.0 ? (u64)(u * 18446744073709551616.0) : ~0ull;
+  };
   // f(l) for this thread's logits l >= least, where few are
   auto each = [&](float least, auto f) {
     for (int q = tid; q < quads; q += ST_THREADS) {
@@ -294,13 +307,13 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
   };
   if (by_count || by_mass) {
     auto clear = [&](int h) {
-      sm.lo[h][tid] = sm.hi[h][tid] = 0;
+      sm.hist[h].lo[tid] = sm.hist[h].hi[tid] = 0;
       __syncthreads();
     };
     auto put = [&](int h, int b, u64 v) {
-      const unsigned low = (unsigned)v, old = atomicAdd(&sm.lo[h][b], low);
+      const unsigned low = (unsigned)v, old = atomicAdd(&sm.hist[h].lo[b], low);
       const unsigned high = (unsigned)(v >> 32) + (old + low < old);
-      if (high) atomicAdd(&sm.hi[h][b], high);
+      if (high) atomicAdd(&sm.hist[h].hi[b], high);
     };
     // The first bin at which the running sum over the cluster's histograms h reaches `want`, -1: none.  The sum before it is added to
     // `before`.
@@ -309,8 +322,8 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
 #pragma unroll
       for (int r = 0; r < ST_MAX_CLUSTER; ++r) {
         const Shared* const o = cl.map_shared_rank(&sm, r < nc ? r : 0);
-        lo[r] = r < nc ? o->lo[h][tid] : 0;
-        hi[r] = r < nc && mass ? o->hi[h][tid] : 0;
+        lo[r] = r < nc ? o->hist[h].lo[tid] : 0;
+        hi[r] = r < nc && mass ? o->hist[h].hi[tid] : 0;
       }
       u64 v = 0;
 #pragma unroll
@@ -323,6 +336,7 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
       if (run < want && run + v >= want) {
         sm.found_bin = tid;
         sm.found_mass = run;
+        sm.found_upto = run + v;
       }
       __syncthreads();
       const int bin = sm.found_bin;
@@ -347,7 +361,7 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
       __syncthreads();
       members([&](float l) {
         if (mass) put(1, sub_step(l), w.of(l));
-        else atomicAdd(&sm.lo[1][sub_step(l)], 1u);
+        else atomicAdd(&sm.hist[1].lo[sub_step(l)], 1u);
       });
       cl.sync();
       const int sub = crossing(1, mass, want, before);
@@ -401,7 +415,7 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
           const unsigned k = key_of(l);
           if (k < k_lo || k > k_hi || sub_step(l) != sub) return;
           if (mass) put(1, (k_hi - k) >> shift, w.of(l));
-          else atomicAdd(&sm.lo[1][(k_hi - k) >> shift], 1u);
+          else atomicAdd(&sm.hist[1].lo[(k_hi - k) >> shift], 1u);
         });
         cl.sync();
         const int s = crossing(1, mass, want, before);
@@ -420,10 +434,67 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
         const float l[4] = {l4.x, l4.y, l4.z, l4.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (l[e] >= least_possible) atomicAdd(&sm.lo[0][(int)w.steps_below(l[e])], 1u);
+          if (l[e] >= least_possible) atomicAdd(&sm.hist[0].lo[(int)w.steps_below(l[e])], 1u);
       }
       cl.sync();
       const int bin = crossing(0, false, (u64)top_k, before);
+      if (bin >= 0 && sm.found_upto <= ST_FEW) {
+        // A small top_k: the first CTA gets everything down to the crossing step and finishes alone, a candidate a thread.  Two
+        // loops over the candidates (what is ahead in the order, what is before in the vocabulary) take the place of all further passes.
+        Shared* const first = cl.map_shared_rank(&sm, 0);
+        u64* const put_few = reinterpret_cast<u64*>(&first->hist[1]);
+        const float down_to = w.surely_below(bin + 1);
+        for (int q = tid; q < quads; q += ST_THREADS) {
+          const float4 l4 = slice4[q];
+          const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+          if (fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) < down_to) continue;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (l[e] >= fmaxf(down_to, least_possible) && (int)w.steps_below(l[e]) <= bin)
+              put_few[atomicAdd(&first->n_list[0], 1)] = ((u64)key_of(l[e]) << 32) | (unsigned)~(base + 4 * q + e - pad);
+        }
+        cl.sync();
+        if (rank == 0) {
+          const u64* const few = reinterpret_cast<const u64*>(&sm.hist[1]);
+          u64* const few_w = reinterpret_cast<u64*>(&sm.hist[0]);
+          const int count = sm.n_list[0];
+          auto block_sum = [&](u64 v) {
+            v = warp_all(v, Add());
+            __syncthreads();
+            if (lane == 0) sm.mass[warp] = v;
+            __syncthreads();
+            return warp_all(lane < ST_WARPS ? sm.mass[lane] : 0, Add());
+          };
+          const u64 mine = tid < count ? few[tid] : 0;
+          u64 v = mine ? w.of(of_key((unsigned)(mine >> 32))) : 0;
+          few_w[tid] = v;
+          __syncthreads();
+          int ahead = 0;
+          u64 run = 0;
+#pragma unroll 4
+          for (int k = 0; k < count; ++k)
+            if (few[k] > mine) {
+              ++ahead;
+              run += few_w[k];
+            }
+          bool keep = mine && ahead < top_k && v >= min_w;
+          if (by_mass) {
+            const u64 want = wanted(block_sum(ahead < top_k ? v : 0));  // by all threads
+            keep = keep && run < want;
+          }
+          v = keep ? v : 0;
+          const u64 all = block_sum(v);
+          few_w[tid] = v;
+          __syncthreads();
+          u64 from = 0;
+#pragma unroll 4
+          for (int k = 0; k < count; ++k) from += (unsigned)few[k] > (unsigned)mine ? few_w[k] : 0;
+          const u64 target = __umul64hi(fraction(), all);
+          if (keep && target >= from && target < from + v) a.out[row] = (long long)(int)~(unsigned)mine;
+        }
+        cl.sync();  // no CTA leaves while another reads its shared memory
+        return;
+      }
       if (bin >= 0) {  // else every possible token is among the first top_k
         cut = narrow(false, (u64)top_k, bin, before);
         ties = (unsigned)((u64)top_k - before);
@@ -449,18 +520,17 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (l[e] >= above) total += v[e];
-          old[e] = l[e] >= put_from ? atomicAdd(&sm.lo[0][(int)w.steps_below(l[e])], (unsigned)v[e]) : 0u;
+          old[e] = l[e] >= put_from ? atomicAdd(&sm.hist[0].lo[(int)w.steps_below(l[e])], (unsigned)v[e]) : 0u;
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const unsigned high = (unsigned)(v[e] >> 32) + (old[e] + (unsigned)v[e] < old[e]);
-          if (l[e] >= put_from && high) atomicAdd(&sm.hi[0][(int)w.steps_below(l[e])], high);
+          if (l[e] >= put_from && high) atomicAdd(&sm.hist[0].hi[(int)w.steps_below(l[e])], high);
         }
       }
       total = cluster_all(cl, nc, sm, total, turn, Add());
       if (counted) total += ties * w(cut);
-      const double some = ceil((top_p > 0.0 ? top_p : 0.0) * (double)total);
-      const u64 want = some >= 1.0 ? (some < (double)total ? (u64)some : total) : 1;
+      const u64 want = wanted(total);
       before = 0;
       const int bin = crossing(0, true, want, before);
       if (bin >= 0) {  // else every token above the cut is needed
@@ -508,7 +578,7 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
   // steps of the first histogram that are kept whole: those above the cut's, whose members are queued; none where min_p cuts higher
   const int whole = by_mass && cut_in ? (int)w.steps_below(cut) : 0;
   if (whole > 0) {
-    u64 m = tid < whole ? ((u64)sm.hi[0][tid] << 32) + sm.lo[0][tid] : 0;
+    u64 m = tid < whole ? ((u64)sm.hist[0].hi[tid] << 32) + sm.hist[0].lo[tid] : 0;
     unsigned eq = 0;
     members([&](float l) {
       if (l >= lower) m += w.of(l);
@@ -533,8 +603,6 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
     }
   }
   cl.sync();
-  double u = a.uniform_f64 ? ((const double*)a.uniform)[row] : (double)((const float*)a.uniform)[row];
-  u = u > 0.0 ? u : 0.0;
   // a lane a CTA of the row; every warp does the same
   const Shared* const o = cl.map_shared_rank(&sm, lane < nc ? lane : 0);
   u64 m = lane < nc ? o->cta_mass : 0;
@@ -542,7 +610,7 @@ __global__ void __launch_bounds__(ST_THREADS, 3) sample_tokens_kernel(SampleArgs
   unsigned tie = warp_before(eq, lane);  // members at the cut before
   if (cut_in && tie < ties) m += min(eq, ties - tie) * cut_w;
   u64 left = warp_before(m, lane);
-  const u64 target = __umul64hi(u < 1.0 ? (u64)(u * 18446744073709551616.0) : ~0ull, __shfl_sync(0xffffffffu, left + m, 31));
+  const u64 target = __umul64hi(fraction(), __shfl_sync(0xffffffffu, left + m, 31));
   const unsigned hit = __ballot_sync(0xffffffffu, target >= left && target < left + m);
   left = target - __shfl_sync(0xffffffffu, left, rank);  // what remains before the target within this CTA, if it is here
   tie = __shfl_sync(0xffffffffu, tie, rank);
