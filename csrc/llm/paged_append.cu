@@ -97,7 +97,7 @@ template <> struct Raw<8> { using V = uint4; };
 // Bound by bytes where there are many tokens: 8192 tokens of 32 + 2 x 8 heads of 128, normalised, move 201 MB in 40 us (5.0 TB/s).
 // Four values a side 46 us, coefficients in shared memory 51 us, a warp a row (the general kernel) 180 us.
 template <typename T, bool INTERLEAVED, int LPR, int SIDE>
-__global__ void __launch_bounds__(AP_WARPS * 32, 5) paged_append_vec_kernel(PagedAppendArgs a, int parts, int* status) {
+__global__ void __launch_bounds__(AP_WARPS * 32, SIDE == 4 ? 8 : 5) paged_append_vec_kernel(PagedAppendArgs a, int parts, int* status) {
   using V = typename Raw<SIDE>::V;
   constexpr int RPW = 32 / LPR, N2 = SIDE / 2;                     // rows of a step, packed pairs of a side
   __shared__ float2 sm_turn[AP_WARPS][LPR * SIDE];
@@ -344,7 +344,11 @@ void paged_append(const PagedAppendArgs& a, cudaStream_t s) {
            even(a.v, a.v_st, a.v_sh) && even(a.q_out, a.qo_st, a.qo_sh) && even(a.k_out, a.ko_st, a.ko_sh) && even(c.k, c.s_page, c.s_head) &&
            even(c.v, c.s_row, 0);
   };
-  if (fits(8)) {
+  // Tokens of few values are bound by the look-ups before their rows, so pieces of four, whose registers let 32 warps an SM run instead
+  // of 20, serve them better (107264 tokens of 8 + 2 heads of 32: 123 us, 162 with eight; 76775 of 4 + 2 of 96 112, 149); tokens of
+  // 32 + 16 heads of 128 40.2 with four, 38.0 with eight; 12 + 24 of 64 alike.
+  const bool light = rows * c.D < 2048 && fits(4);
+  if (!light && fits(8)) {
     if (a.dtype == DT_F16) launch_vec_order<__half, 8>(a, status, s);
     else launch_vec_order<__nv_bfloat16, 8>(a, status, s);
   } else if (fits(4)) {
