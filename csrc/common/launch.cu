@@ -78,10 +78,15 @@ int* status_word(int device) {
   if (!g_status[device]) {
     int prev = current_device();
     RT_CUDA_CHECK(cudaSetDevice(device));
+    // the first call of a process may come inside a graph capture, whose thread may not allocate unless it says so
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    RT_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
     int* p = nullptr;
-    RT_CUDA_CHECK(cudaMalloc(&p, sizeof(int) * 16));
-    RT_CUDA_CHECK(cudaMemset(p, 0, sizeof(int) * 16));
+    cudaError_t err = cudaMalloc(&p, sizeof(int) * 16);
+    if (err == cudaSuccess) err = cudaMemset(p, 0, sizeof(int) * 16);
+    RT_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
     RT_CUDA_CHECK(cudaSetDevice(prev));
+    RT_CUDA_CHECK(err);
     g_status[device] = p;
   }
   return g_status[device];

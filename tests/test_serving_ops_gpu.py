@@ -1,5 +1,8 @@
 """Paged cache append, paged attention and token sampling kernels against their 64-bit definitions."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -367,6 +370,34 @@ def test_captured_and_eager_calls_at_once():
     torch.cuda.synchronize()
     assert torch.equal(captured, want[0])
     assert all(torch.equal(x, want[1]) for x in got[0]) and all(torch.equal(x, want[2]) for x in got[1])
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    """Nothing has to run before a capture: what the kernels allocate once per process is allocated there."""
+    code = """
+import torch
+from rustorch_b200 import _native
+from rustorch_b200.ops.paged import paged_append, paged_attention
+from rustorch_b200.ops.sampling import sample_tokens
+x = torch.randn(1, 2, 64, device="cuda").half()
+kp, vp = torch.zeros(2, 2, 16, 64, device="cuda").half(), torch.zeros(2, 2, 16, 64, device="cuda").half()
+i = torch.zeros(1, dtype=torch.int32, device="cuda")
+table, inv, u, one = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.ones(32, device="cuda"), torch.full((1,), 0.5, device="cuda"), i + 1
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    q = paged_append(x, x, x, kp, vp, table, i, i, inv)
+    out = paged_attention(q, kp, vp, table, one, i)
+    tok = sample_tokens(out.flatten(1), u, temperature=0.0)
+g.replay()
+torch.cuda.synchronize()
+_native.check_status()
+assert torch.equal(out, x) and int(tok) == int(x.argmax())
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-800:]
 
 
 def test_empty_calls():
