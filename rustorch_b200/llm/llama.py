@@ -567,6 +567,24 @@ class LlamaRuntime:
         return logits
 
     # ----------------------------------------------------------- CUDA-graph decode
+    def _shared_numbers(self, uniform: torch.Tensor) -> torch.Tensor:
+        """The random numbers of the group's first rank, on the device.  Tensor-parallel ranks that drew by numbers of their own
+        would go on with different tokens and add activations of different sequences."""
+        uniform = uniform.to(self.device)
+        if self.tp_world > 1:
+            uniform = uniform.clone(memory_format=torch.contiguous_format)
+            dist.broadcast(uniform, dist.get_global_rank(self.tp_group, 0) if self.tp_group is not None else 0, group=self.tp_group)
+        return uniform
+
+    def _numbers(self, sampling: SamplingConfig, steps: int, batch: int, uniform: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``[steps, batch]`` numbers to draw by: ``uniform``, or numbers from ``sampling.seed`` (without one, the host's generator)."""
+        if uniform is None:
+            gen = torch.Generator().manual_seed(sampling.seed) if sampling.seed is not None else None
+            uniform = torch.rand(steps, batch, generator=gen)
+        if uniform.shape != (steps, batch):
+            raise ValueError(f"uniform must be [{steps}, {batch}], got {list(uniform.shape)}")
+        return self._shared_numbers(uniform)
+
     @torch.no_grad()
     def capture_decode_graph(self, cache: Union[KVCache, PagedKVCache], batch: int, sampling: Optional[SamplingConfig] = None,
                              uniform: Optional[torch.Tensor] = None) -> "_DecodeGraph":
@@ -574,8 +592,8 @@ class LlamaRuntime:
         graph whose inputs live on the device: a step is then one graph launch, and the ~10 launches per
         layer no longer pay host latency.  Positions and the current tokens are device tensors that the graph
         itself advances, so replaying it N times generates N tokens without any host round trip.  With ``sampling``
-        step ``i`` draws its tokens by row ``i`` of ``uniform [steps, batch]`` instead of taking the most likely ones.  The pages of a
-        paged cache have to be reserved before."""
+        step ``i`` draws its tokens by row ``i`` of ``uniform [steps, batch]`` instead of taking the most likely ones (tensor-parallel
+        ranks all by the first rank's).  The pages of a paged cache have to be reserved before."""
         dev = self.device
         g = _DecodeGraph()
         if sampling is not None:
@@ -584,7 +602,7 @@ class LlamaRuntime:
                 raise ValueError("a captured decode step keeps no history: repetition_penalty must be 1")
             if uniform is None or uniform.dim() != 2 or uniform.shape[1] != batch:
                 raise ValueError("sampling needs random numbers, uniform [steps, batch]")
-            g.uniform = uniform.to(dev)
+            g.uniform = self._shared_numbers(uniform)
         g.tok = torch.zeros(batch, dtype=torch.long, device=dev)
         g.pos = torch.zeros(batch, dtype=torch.int32, device=dev)
         g.seq = torch.arange(batch, dtype=torch.int32, device=dev)
@@ -621,7 +639,8 @@ class LlamaRuntime:
                        ) -> Tuple[torch.Tensor, Dict[str, float]]:
         """Greedy generation with the decode loop replayed from a CUDA graph (single process or TP ranks that
         all call it together).  Same outputs as ``generate`` without a sampler.  With ``sampling`` the tokens are drawn on the
-        device by ``uniform [max_new_tokens, B]`` (row 0: the token after the prompt), by default numbers from ``sampling.seed``."""
+        device by ``uniform [max_new_tokens, B]`` (row 0: the token after the prompt), by default numbers from ``sampling.seed``;
+        tensor-parallel ranks all draw by the first rank's numbers."""
         B, T = prompts.shape
         cache = cache or self.new_cache(B, T + max_new_tokens)
         dev = self.device
@@ -629,12 +648,7 @@ class LlamaRuntime:
             for b in range(B):
                 cache.reserve(b, T + max_new_tokens)
         if sampling is not None:
-            if uniform is None:
-                gen = torch.Generator().manual_seed(sampling.seed) if sampling.seed is not None else None
-                uniform = torch.rand(max_new_tokens, B, generator=gen)
-            if uniform.shape != (max_new_tokens, B):
-                raise ValueError(f"uniform must be [{max_new_tokens}, {B}], got {list(uniform.shape)}")
-            uniform = uniform.to(dev)
+            uniform = self._numbers(sampling, max_new_tokens, B, uniform)
         # the warm-up/capture writes only at position 0.. (reset below)
         g = self.capture_decode_graph(cache, B, sampling, uniform[1:] if uniform is not None and max_new_tokens > 1 else uniform)
         torch.cuda.synchronize(dev)
