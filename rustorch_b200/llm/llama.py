@@ -124,7 +124,7 @@ class PagedKVCache:
         return self.lengths[b]
 
     def clear(self) -> None:
-        for b in range(len(self.lengths)):
+        for b in range(len(self.pages)):
             self.release(b)
 
     def nbytes(self) -> int:
@@ -538,7 +538,8 @@ class LlamaRuntime:
     # --------------------------------------------------------------- generate
     @torch.no_grad()
     def prefill(self, prompts: torch.Tensor, cache: KVCache) -> torch.Tensor:
-        """``prompts [B, T]`` (equal lengths) -> logits of the last position ``[B, vocab]``."""
+        """``prompts [B, T]`` (equal lengths) -> logits of the last position ``[B, vocab]``.  Fills the cache's first ``B`` sequences from
+        their start; the others stay."""
         B, T = prompts.shape
         dev = self.device
         if isinstance(cache, PagedKVCache):
@@ -549,21 +550,22 @@ class LlamaRuntime:
         seq = torch.arange(B, device=dev).repeat_interleave(T)
         last = torch.arange(B, device=dev) * T + (T - 1)
         logits = self.forward_tokens(tokens, pos, seq, cache, last_only=last, max_kv=T, prefill_bt=(B, T))
-        cache.lengths = [T] * B
+        cache.lengths[:B] = [T] * B                            # the cache may hold more sequences
         return logits
 
     @torch.no_grad()
     def decode_step(self, tokens: torch.Tensor, cache: KVCache) -> torch.Tensor:
-        """One new token per sequence: ``tokens [B]`` -> logits ``[B, vocab]``."""
+        """One new token for each of the cache's first ``B`` sequences: ``tokens [B]`` -> logits ``[B, vocab]``."""
         B = tokens.shape[0]
         dev = self.device
         if isinstance(cache, PagedKVCache):
             for b in range(B):
                 cache.reserve(b, cache.lengths[b] + 1)
-        pos = torch.tensor(cache.lengths, device=dev)
+        lengths = cache.lengths[:B]
+        pos = torch.tensor(lengths, device=dev)
         seq = torch.arange(B, device=dev)
-        logits = self.forward_tokens(tokens.to(dev), pos, seq, cache, max_kv=max(cache.lengths) + 1)
-        cache.lengths = [l + 1 for l in cache.lengths]
+        logits = self.forward_tokens(tokens.to(dev), pos, seq, cache, max_kv=max(lengths) + 1)
+        cache.lengths[:B] = [l + 1 for l in lengths]
         return logits
 
     # ----------------------------------------------------------- CUDA-graph decode
@@ -670,7 +672,7 @@ class LlamaRuntime:
             g.graph.replay()
         torch.cuda.synchronize(dev)
         dt = time.perf_counter() - t1
-        cache.lengths = [T + steps] * B
+        cache.lengths[:B] = [T + steps] * B
         toks = torch.cat([prompts.to(dev), nxt.view(B, 1), g.out[:, :steps]], 1)
         return toks, {"ttft_s": ttft, "decode_tokens_per_s": B * steps / dt if dt > 0 and steps else 0.0,
                       "decode_steps": steps, "batch": B}
