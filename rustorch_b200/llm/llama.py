@@ -82,8 +82,8 @@ class KVCache:
 
 class PagedKVCache:
     """Key/value cache in pages ``[n_pages, Hkv_local, page, D]`` per layer that the sequences share: a sequence holds the pages its
-    positions need (``reserve``) and gives them back (``release``), so memory follows the lengths in use instead of
-    ``batch * max_len``.  ``block_table [batch, ceil(max_len / page)]`` (int32, on the device) names a sequence's pages, -1 where
+    positions need (``reserve``) and gives them back (``release``; it is idle then, until pages are reserved for it again), so memory
+    follows the lengths in use instead of ``batch * max_len``.  ``block_table [batch, ceil(max_len / page)]`` (int32, on the device) names a sequence's pages, -1 where
     it has none.  ``n_pages`` defaults to what ``batch`` sequences of ``max_len`` need."""
 
     def __init__(self, n_layer: int, batch: int, n_head_kv: int, max_len: int, head_dim: int, device, dtype=torch.float16, page: int = 64,
@@ -99,11 +99,13 @@ class PagedKVCache:
         self.pages: List[List[int]] = [[] for _ in range(batch)]
         self.free = list(range(self.n_pages - 1, -1, -1))
         self.lengths = [0] * batch
+        self.idle = [False] * batch                            # released: decode steps pass it over
 
     def reserve(self, b: int, length: int) -> None:
         """Gives sequence ``b`` pages for positions ``0 .. length - 1``; those it has stay."""
         if length > self.max_len:
             raise ValueError(f"{length} positions exceed the cache's limit of {self.max_len}")
+        self.idle[b] = self.idle[b] and length < 1
         have, need = len(self.pages[b]), (length + self.page - 1) // self.page
         if need <= have:
             return
@@ -114,18 +116,21 @@ class PagedKVCache:
         self.block_table[b, have:need] = torch.tensor(new, dtype=torch.int32).to(self.block_table.device)
 
     def release(self, b: int) -> None:
-        """Takes all pages of sequence ``b`` back and forgets its contents."""
+        """Takes all pages of sequence ``b`` back and forgets its contents.  It is idle until ``reserve`` or a prompt gives it pages."""
         self.free += reversed(self.pages[b])
         self.pages[b] = []
         self.block_table[b].fill_(-1)
         self.lengths[b] = 0
+        self.idle[b] = True
 
     def seq_len(self, b: int = 0) -> int:
         return self.lengths[b]
 
     def clear(self) -> None:
+        """Back to a new cache: every sequence is empty and starts with its next token."""
         for b in range(len(self.pages)):
             self.release(b)
+            self.idle[b] = False
 
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in self.k + self.v)
@@ -555,17 +560,20 @@ class LlamaRuntime:
 
     @torch.no_grad()
     def decode_step(self, tokens: torch.Tensor, cache: KVCache) -> torch.Tensor:
-        """One new token for each of the cache's first ``B`` sequences: ``tokens [B]`` -> logits ``[B, vocab]``."""
+        """One new token for each of the cache's first ``B`` sequences: ``tokens [B]`` -> logits ``[B, vocab]``.  A released sequence
+        of a paged cache is passed over: its token is ignored, its logits mean nothing, and it takes no page."""
         B = tokens.shape[0]
         dev = self.device
+        lengths, idle = cache.lengths[:B], [False] * B
         if isinstance(cache, PagedKVCache):
+            idle = cache.idle[:B]
             for b in range(B):
-                cache.reserve(b, cache.lengths[b] + 1)
-        lengths = cache.lengths[:B]
+                if not idle[b]:
+                    cache.reserve(b, lengths[b] + 1)
         pos = torch.tensor(lengths, device=dev)
-        seq = torch.arange(B, device=dev)
+        seq = torch.tensor([-1 if x else b for b, x in enumerate(idle)], device=dev) if any(idle) else torch.arange(B, device=dev)
         logits = self.forward_tokens(tokens.to(dev), pos, seq, cache, max_kv=max(lengths) + 1)
-        cache.lengths[:B] = [l + 1 for l in lengths]
+        cache.lengths[:B] = [l + (not x) for l, x in zip(lengths, idle)]
         return logits
 
     # ----------------------------------------------------------- CUDA-graph decode

@@ -52,3 +52,48 @@ def test_clear_gives_back_pages_of_sequences_that_no_call_covered():
     assert sorted(cache.free) == list(range(32))
     cache.release(3)
     assert cache.lengths == [0] * 4
+
+
+def test_a_released_sequence_sits_out_until_it_is_reserved_again():
+    rt = _runtime()
+    prompt, tok = _prompt(4, 9), torch.tensor([5, 6, 7, 8])
+    cache, plain = rt.new_paged_cache(4, 32, page=3, n_pages=17), rt.new_cache(4, 32)
+    rt.prefill(prompt, cache), rt.prefill(prompt, plain)
+    cache.release(1)
+    before = [k.clone() for k in cache.k]
+    taken = [list(p) for p in cache.pages]
+    for step in range(3):                                      # a pool that the others need for themselves
+        out, want = rt.decode_step(tok, cache), rt.decode_step(tok, plain)
+        assert torch.allclose(out[[0, 2, 3]], want[[0, 2, 3]], rtol=1e-4, atol=1e-4) and bool(torch.isfinite(out).all())
+        assert cache.lengths == [10 + step, 0, 10 + step, 10 + step] and cache.pages[1] == []
+    for k, old in zip(cache.k, before):                        # nothing was written to pages that nobody holds
+        for page in cache.free:
+            assert torch.equal(k[page], old[page])
+    assert cache.pages[0][:3] == taken[0] and len(cache.free) == 17 - 3 * 4
+    # its place is taken by another sequence, fed by hand
+    new = _prompt(1, 5, seed=2)[0]
+    cache.reserve(1, 5)
+    pos = torch.arange(5)
+    rt.forward_tokens(new, pos, torch.full_like(pos, 1), cache)
+    cache.lengths[1] = 5
+    out = rt.decode_step(tok, cache)
+    fresh = rt.new_cache(1, 32)
+    rt.prefill(new[None], fresh)
+    assert torch.allclose(out[1], rt.decode_step(tok[1:2], fresh)[0], rtol=1e-4, atol=1e-4)
+    assert cache.lengths == [13, 6, 13, 13]
+
+
+def test_a_released_batch_is_filled_by_the_next_prompt_and_a_cleared_one_starts_anew():
+    rt = _runtime()
+    prompt, tok = _prompt(2, 7), torch.tensor([5, 6])
+    cache = rt.new_paged_cache(2, 32, page=4)
+    for _ in range(2):
+        rt.prefill(prompt, cache)
+        assert rt.decode_step(tok, cache).shape == (2, 97) and cache.lengths == [8, 8]
+        cache.release(0), cache.release(1)
+    assert rt.decode_step(tok, cache).shape == (2, 97) and cache.lengths == [0, 0] and len(cache.free) == cache.n_pages
+    cache.clear()                                              # like a new cache, whose sequences start at position 0 with their first step
+    plain = rt.new_cache(2, 32)
+    for _ in range(2):
+        assert torch.allclose(rt.decode_step(tok, cache), rt.decode_step(tok, plain), rtol=1e-4, atol=1e-4)
+    assert cache.lengths == [2, 2]
