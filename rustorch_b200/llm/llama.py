@@ -656,7 +656,7 @@ class LlamaRuntime:
         dev = self.device
         if isinstance(cache, PagedKVCache):
             for b in range(B):
-                cache.reserve(b, T + max_new_tokens)
+                cache.reserve(b, T + max(0, max_new_tokens - 1))       # the last token is not appended
         if sampling is not None:
             uniform = self._numbers(sampling, max_new_tokens, B, uniform)
         # the warm-up/capture writes only at position 0.. (reset below)
