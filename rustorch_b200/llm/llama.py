@@ -603,15 +603,16 @@ class LlamaRuntime:
         layer no longer pay host latency.  Positions and the current tokens are device tensors that the graph
         itself advances, so replaying it N times generates N tokens without any host round trip.  With ``sampling``
         step ``i`` draws its tokens by row ``i`` of ``uniform [steps, batch]`` instead of taking the most likely ones (tensor-parallel
-        ranks all by the first rank's).  The pages of a paged cache have to be reserved before."""
+        ranks all by the first rank's); further replays use the last row again and write over its step's place in ``out``.  The pages
+        of a paged cache have to be reserved before."""
         dev = self.device
         g = _DecodeGraph()
         if sampling is not None:
             sampling.validate()
             if sampling.repetition_penalty != 1.0:
                 raise ValueError("a captured decode step keeps no history: repetition_penalty must be 1")
-            if uniform is None or uniform.dim() != 2 or uniform.shape[1] != batch:
-                raise ValueError("sampling needs random numbers, uniform [steps, batch]")
+            if uniform is None or uniform.dim() != 2 or uniform.shape[0] < 1 or uniform.shape[1] != batch:
+                raise ValueError("sampling needs random numbers, uniform [steps, batch] with one step at least")
             g.uniform = self._shared_numbers(uniform)
         g.tok = torch.zeros(batch, dtype=torch.long, device=dev)
         g.pos = torch.zeros(batch, dtype=torch.int32, device=dev)
@@ -630,6 +631,8 @@ class LlamaRuntime:
             g.tok.copy_(nxt)
             g.pos.add_(1)
             g.step.add_(1)
+            if sampling is not None:                           # replays beyond the numbers use the last row again, none reads behind it
+                g.step.clamp_(max=min(g.uniform.shape[0], cache.max_len) - 1)
             return logits
 
         side = torch.cuda.Stream(device=dev)

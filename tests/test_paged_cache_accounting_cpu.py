@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from rustorch_b200.llm import LlamaConfig, LlamaRuntime
+from rustorch_b200.llm import LlamaConfig, LlamaRuntime, SamplingConfig
 
 
 def _runtime(**kw):
@@ -97,3 +97,10 @@ def test_a_released_batch_is_filled_by_the_next_prompt_and_a_cleared_one_starts_
     for _ in range(2):
         assert torch.allclose(rt.decode_step(tok, cache), rt.decode_step(tok, plain), rtol=1e-4, atol=1e-4)
     assert cache.lengths == [2, 2]
+
+
+def test_captured_sampling_without_numbers_is_refused():
+    rt = _runtime()
+    for bad in (None, torch.zeros(0, 2), torch.zeros(3, 4), torch.zeros(2)):
+        with pytest.raises(ValueError, match="random numbers"):
+            rt.capture_decode_graph(rt.new_paged_cache(2, 32), 2, SamplingConfig(), bad)

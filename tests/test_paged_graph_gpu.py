@@ -25,3 +25,29 @@ def test_graph_generation_fits_a_cache_without_a_place_for_the_last_token(new):
     _native.check_status()
     assert torch.equal(got, rt.generate_graph(prompt, new, cache=rt.new_paged_cache(3, 128))[0])
     assert tight.lengths == [24 + new - 1] * 3 and tight.free == []
+
+
+def test_replays_beyond_the_numbers_use_the_last_row():
+    """Four rows of numbers, seven replays: the last ones draw by the fourth row and stay in its place of the output."""
+    from rustorch_b200 import _native
+    from rustorch_b200.llm import SamplingConfig
+    rt, prompt = _runtime(), _prompt(2, 5)
+    cfg, u = SamplingConfig(temperature=1.1, top_p=0.95), torch.rand(4, 2, generator=torch.Generator().manual_seed(1))
+
+    def decode(numbers, replays):
+        cache = rt.new_paged_cache(2, 64, page=8)
+        cache.reserve(0, 20), cache.reserve(1, 20)
+        g = rt.capture_decode_graph(cache, 2, cfg, numbers)
+        logits = rt.prefill(prompt, cache)
+        g.tok.copy_(logits.argmax(-1)), g.pos.fill_(5), g.step.zero_()
+        for _ in range(replays):
+            g.graph.replay()
+        torch.cuda.synchronize()
+        _native.check_status()
+        return g.out.cpu(), g.tok.cpu(), int(g.step)
+    out, tok, step = decode(u, 7)
+    long_out, long_tok, _ = decode(torch.cat([u, u[3:].expand(3, -1)]), 7)       # the same numbers, spelled out
+    assert step == 3 and torch.equal(out[:, :3], long_out[:, :3]) and torch.equal(tok, long_tok)
+    assert torch.equal(out[:, 3], long_out[:, 6]) and int(out[:, 4:].abs().sum()) == 0
+    exact, _, _ = decode(u, 4)
+    assert torch.equal(exact[:, :4], long_out[:, :4])
