@@ -41,12 +41,16 @@ def softmax(logits: torch.Tensor) -> torch.Tensor:
 
 
 def apply_repetition_penalty(logits: torch.Tensor, history: torch.Tensor, penalty: float) -> torch.Tensor:
-    """Divide positive / multiply negative logits of already generated tokens by ``penalty``."""
+    """Divide positive / multiply negative logits of already generated tokens by ``penalty``.  Entries below zero stand for steps that
+    had no token (``Sampler.draw``) and change nothing."""
     if penalty == 1.0 or history.numel() == 0:
         return logits
     out = logits.clone()
-    g = out.gather(-1, history)
-    out.scatter_(-1, history, torch.where(g > 0, g / penalty, g * penalty))
+    token = history.clamp_min(0)
+    g = out.gather(-1, token)
+    # a missing token is sent to place 0 with what that place gets anyway, so that all writers of a place agree
+    keep = (history < 0) & ~(history == 0).any(-1, keepdim=True)
+    out.scatter_(-1, token, torch.where(keep, g, torch.where(g > 0, g / penalty, g * penalty)))
     return out
 
 
