@@ -382,15 +382,28 @@ class LlamaRuntime:
         xf = x.float()
         return (xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + self.cfg.rms_eps) * w.float()).to(x.dtype)
 
+    def _build_inv_freq(self, D: int, device) -> torch.Tensor:
+        inv = self.cfg.rope_theta ** (-torch.arange(D // 2, device=device, dtype=torch.float32) * 2.0 / D)
+        if self.cfg.rope_scaling:
+            from ..models.llama import scale_rope_frequencies
+            inv = scale_rope_frequencies(inv, self.cfg.rope_scaling)
+        return inv
+
     def _inv_freq(self, D: int, device) -> torch.Tensor:
-        """Rotation frequencies of the ``D // 2`` pairs, with the checkpoint's frequency scaling applied."""
+        """Rotation frequencies of the ``D // 2`` pairs, with the checkpoint's frequency scaling applied; made once a device."""
+        device = torch.device(device)
         cached = getattr(self, "_inv_freq_cache", None)
-        if cached is None or cached.shape[0] != D // 2 or cached.device != torch.device(device):
-            cached = self.cfg.rope_theta ** (-torch.arange(D // 2, device=device, dtype=torch.float32) * 2.0 / D)
-            if self.cfg.rope_scaling:
-                from ..models.llama import scale_rope_frequencies
-                cached = scale_rope_frequencies(cached, self.cfg.rope_scaling)
-            self._inv_freq_cache = cached
+        if device.type == "cuda":
+            if device.index is None:
+                device = torch.device("cuda", torch.cuda.current_device())
+            if cached is not None and cached.shape[0] == D // 2 and cached.device == device:
+                return cached
+            if torch.cuda.is_current_stream_capturing():       # the graph's memory, filled by its replays alone
+                return self._build_inv_freq(D, device)
+            self._inv_freq_cache = cached = self._build_inv_freq(D, device)
+            torch.cuda.current_stream(device).synchronize()    # later calls may come on other streams
+        elif cached is None or cached.shape[0] != D // 2 or cached.device != device:
+            self._inv_freq_cache = cached = self._build_inv_freq(D, device)
         return cached
 
     def _rope_reference(self, t: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
