@@ -133,9 +133,10 @@ __global__ void reduce_kernel(const T* __restrict__ x, float* __restrict__ out, 
 // out must be pre-initialised by the caller (0 for sums, -inf / +inf for max / min).
 void reduce_all(const void* x, int dtype, int mode, float* out, long long n, cudaStream_t stream) {
   if (n == 0) return;
-  // Up to 32768 values (the row losses of a training step) one CTA adds them in a fixed order: the atomics of several
-  // would make the last bits of a loss depend on which of them came first.
-  const bool one = n <= 32768;
+  // Sums of up to 32768 values (the row losses of a training step) are added by one CTA in a fixed order: the atomics of several
+  // would make the last bits of a loss depend on which of them came first.  2048 values take 1.95 us (1.6 with eight CTAs), 8192
+  // 2.0 (1.7), 32768 3.2 (1.7).  Maxima are the same in any order and take several.
+  const bool one = n <= 32768 && mode <= 1;
   const int threads = one ? 1024 : 256;
   const int grid = one ? 1 : (int)std::min<long long>((n + threads - 1) / threads, 4LL * sm_count(current_device()));
 #define RT_RED(T, M) reduce_kernel<T, M><<<grid, threads, 0, stream>>>(reinterpret_cast<const T*>(x), out, n)
