@@ -20,6 +20,14 @@ using OptTensor = c10::optional<Tensor>;
 cudaStream_t stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
 
+void no_gradients(const char* op, std::initializer_list<const Tensor*> required, std::initializer_list<const OptTensor*> optional) {
+  if (!at::GradMode::is_enabled()) return;
+  bool asks = false;
+  for (const Tensor* t : required) asks |= t->requires_grad();
+  for (const OptTensor* t : optional) asks |= given(*t) && (*t)->requires_grad();
+  if (asks) throw pybind11::value_error(std::string(op) + " has no backward pass: call it under torch.no_grad()");
+}
+
 int dtype16(const Tensor& t, const char* op) {
   if (t.scalar_type() == at::kHalf) return rt::DT_F16;
   TORCH_CHECK(t.scalar_type() == at::kBFloat16, op, ": fp16 or bf16 CUDA tensors required");
@@ -77,6 +85,7 @@ Tensor paged_append(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
                     const Tensor& pos, const OptTensor& seq, const Tensor& inv_freq, bool interleaved, const OptTensor& q_norm,
                     const OptTensor& k_norm, double eps, const OptTensor& q_out, const OptTensor& k_out) {
   const char* op = "paged_append";
+  no_gradients(op, {&q, &k, &v, &k_pages, &v_pages, &inv_freq}, {&q_norm, &k_norm, &q_out, &k_out});
   rt::PagedAppendArgs a{};
   a.dtype = dtype16(k_pages, op);
   a.cache = make_cache(k_pages, v_pages, table, op);
@@ -150,6 +159,7 @@ Tensor attention_workspace(const Tensor& like, int64_t bytes) {
 Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& kv_len,
                        const OptTensor& seq, double scale, int64_t window, double softcap, const OptTensor& out_) {
   const char* op = "paged_attention";
+  no_gradients(op, {&q_in, &k_pages, &v_pages}, {&out_});
   rt::PagedAttnArgs a{};
   a.dtype = dtype16(k_pages, op);
   a.cache = make_cache(k_pages, v_pages, table, op);

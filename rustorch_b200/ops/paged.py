@@ -20,11 +20,6 @@ import torch
 from .. import _native
 
 
-def _no_gradients(op, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{op} has no backward pass: call it under torch.no_grad()")
-
-
 def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                  block_table: torch.Tensor, pos: torch.Tensor, seq: Optional[torch.Tensor], inv_freq: torch.Tensor, *,
                  interleaved: bool = False, q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None,
@@ -38,8 +33,8 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
     to every head before the rotation.  ``q_out`` may be ``q`` itself, ``k_out`` (the rotated keys, also in the
     cache) ``k`` itself; other overlaps of inputs and outputs are not allowed.  Inference only: inputs that ask for gradients are refused.
     """
-    _no_gradients("paged_append", q, k, v, k_pages, v_pages, inv_freq, q_norm, k_norm, q_out, k_out)
     if k_pages.device.type == "cpu":
+        _no_gradients("paged_append", q, k, v, k_pages, v_pages, inv_freq, q_norm, k_norm, q_out, k_out)
         return _append_cpu(q, k, v, k_pages, v_pages, block_table, pos, seq, inv_freq, interleaved, q_norm, k_norm, eps, q_out, k_out)
     return _native.load(required=True).paged_append(q, k, v, k_pages, v_pages, block_table, pos, seq, inv_freq, interleaved, q_norm,
                                                     k_norm, eps, q_out, k_out)
@@ -55,12 +50,17 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``f(x) = softcap tanh(x / softcap)`` (1e-6 to 1e30); ``scale`` defaults to ``1 / sqrt(D)``.  A token that sees no position gets zeros.
     What the cache holds beyond the visible positions (NaN included) does not matter.  Inference only: inputs that ask for gradients are refused.
     """
-    _no_gradients("paged_attention", q, k_pages, v_pages, out)
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     if k_pages.device.type == "cpu":
+        _no_gradients("paged_attention", q, k_pages, v_pages, out)
         return _attention_cpu(q, k_pages, v_pages, block_table, kv_len, seq, scale, window, softcap, out)
     return _native.load(required=True).paged_attention(q, k_pages, v_pages, block_table, kv_len, seq, scale, window, softcap, out)
+
+
+def _no_gradients(op, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{op} has no backward pass: call it under torch.no_grad()")
 
 
 def _check_cpu(op, k_pages, v_pages, block_table, n, **indices):
