@@ -19,8 +19,8 @@
 // values as two groups, refilled one after the other, 118 us; a window of 32 block-table entries in registers 100 us.
 // The products are m16n8k16 with the cache as the 16 rows and eight query heads as the columns: S^T = K Q^T (16 keys),
 // O^T += V^T P^T (16 of D).  Decode has 1 to 16 query heads a kv head, a corner of a 128-row tcgen05 tile; here the tensor
-// time is a fraction of the load time.  Weights enter the second product as two values of the cache's type, the rounded weight and
-// what that rounding left, 16 bits together in bf16 and 22 in fp16: the result's own rounding is then the only one of its size
+// time is a fraction of the load time.  Weights enter the second product as two values of the cache's type, what fits the
+// first and what that left, 16 bits together in bf16 and 22 in fp16: the result's own rounding is then the only one of its size
 // (131072 keys take 96.6 us, 95.8 with weights rounded once; 64 sequences of 1 to 8192 keys in fp16 141 and 137).
 // Rows that are not visible are not copied: a tile that has some masks their scores, and their values too, which may be left-over NaN.
 // Maximum, sum and output are kept in 32 bits.
@@ -93,9 +93,20 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return pack_2x16<std::is_same<T, __half>::value>(lo, hi); }
-template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t r) {
-  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&r));
-  else return make_float2(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
+// Two weights as sums of two values of type T, packed: the first is cut off strictly below the weight, so that the second is positive
+// too and an infinite value times a weight stays infinite.  (fp16 cannot hold a second part below 2^-24: weights from 2^-10 on, of 2^4
+// and more for the largest, get that.)
+template <typename T> __device__ __forceinline__ void split2(float a, float b, uint32_t& first, uint32_t& second) {
+  const uint32_t x = __float_as_uint(fmaxf(a, 1.17549435e-38f)) - 1, y = __float_as_uint(fmaxf(b, 1.17549435e-38f)) - 1;
+  if constexpr (std::is_same<T, __half>::value) {
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(first) : "f"(__uint_as_float(y)), "f"(__uint_as_float(x)));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&first));
+    const float r = a - f.x, s = b - f.y;
+    second = pack2<T>(a >= 0x1p-10f ? fmaxf(r, 0x1p-24f) : r, b >= 0x1p-10f ? fmaxf(s, 0x1p-24f) : s);
+  } else {
+    first = __byte_perm(x, y, 0x7632);
+    second = pack2<T>(a - __uint_as_float(x & 0xffff0000u), b - __uint_as_float(y & 0xffff0000u));
+  }
 }
 __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half(v); }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
@@ -406,7 +417,7 @@ paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, bool 
               }
             }
         }
-        uint32_t p[NH][2], rest[NH][2];  // weights: rounded to the values' type, and what the rounding left, rounded again
+        uint32_t p[NH][2], rest[NH][2];  // the weights' two parts
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
 #pragma unroll
@@ -415,10 +426,10 @@ paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, bool 
           l[h][1] += s[h][0][1] + s[h][0][3];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const uint32_t w = pack2<T>(s[h][0][2 * e], s[h][0][2 * e + 1]);
-            const float2 f = unpack2<T>(w);
+            uint32_t w, r;
+            split2<T>(s[h][0][2 * e], s[h][0][2 * e + 1], w, r);
             p[h][e] = transpose8x8(w);
-            rest[h][e] = transpose8x8(pack2<T>(s[h][0][2 * e] - f.x, s[h][0][2 * e + 1] - f.y));
+            rest[h][e] = transpose8x8(r);
           }
         }
         const int kk = 2 * (lane & 3);

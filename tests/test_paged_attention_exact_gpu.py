@@ -122,3 +122,27 @@ def test_every_key_of_a_ragged_batch_counts_once(seed):
             want = torch.bincount(marks, minlength=D).double() / max(1, n)
             # sums of equal weights are exact: the division and the result's rounding are left
             assert bool(((out[t, h] - want).abs() <= want * (half_step(torch.float16) + 2 * 2.0 ** -24) + 2.0 ** -25).all()), (t, h)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("scale", [0.0, 0.1])
+@pytest.mark.parametrize("heads,D", [(1, 64), (12, 128), (2, 256)])
+def test_infinite_values_stay_infinite(dtype, scale, heads, D):
+    """Keys of a few different weights (equal ones with scale 0); some values of one sign are infinite: so is the answer in their place,
+    and finite everywhere else.  NaN and infinities of both signs give NaN."""
+    from rustorch_b200.ops.paged import paged_attention
+    g = torch.Generator().manual_seed(D)
+    n = 3000
+    keys, values = torch.randn(n, D, generator=g), torch.randn(n, D, generator=g)
+    at = torch.randint(0, n, (D,), generator=g)
+    for d in range(D):
+        if d % 4:
+            values[at[d], d] = (float("inf"), -float("inf"), float("nan"))[d % 4 - 1]
+        if d % 8 == 5:
+            values[(at[d] + 100) % n, d] = -float("inf")
+    q = torch.randn(1, heads, D, generator=g).to(dtype)
+    out = paged_attention(q.cuda(), *_pages(keys, values, 16, dtype), _i32([n]), scale=scale).float().cpu()[0]
+    for d in range(D):
+        want = ("finite", "inf", "-inf", "nan")[d % 4] if d % 8 != 5 else "nan"
+        got = out[:, d]
+        assert bool({"finite": torch.isfinite(got), "inf": got == float("inf"), "-inf": got == -float("inf"), "nan": torch.isnan(got)}[want].all()), (d, want)
