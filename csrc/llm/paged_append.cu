@@ -94,7 +94,8 @@ template <> struct Raw<8> { using V = uint4; };
 // pairs are the same for every head, so its coefficients (cosine and sine times the norm's weights) stay in registers:
 //   a <- r (a wa cos - b wb sin),  b <- r (a wa sin + b wb cos),  r = rsqrt(mean + eps) or 1
 // in packed 32-bit pairs.  Cosines and sines are computed once a warp, one pair a lane at a time, while the first rows load.
-// Bound by bytes where there are many tokens: 8192 tokens of 32 + 2 x 8 heads of 128, normalised, move 201 MB in 40 us (5.0 TB/s).
+// Bound by bytes where there are many tokens, with waits for loads beside (2.8 waves of CTAs): 8192 tokens of 32 + 2 x 8 heads of 128,
+// normalised, move 201 MB in 40 us (5.0 TB/s, 0.76 of a plain copy's rate).
 // Four values a side 43 us, coefficients in shared memory 51 us, a warp a row (the general kernel) 180 us.
 template <typename T, bool INTERLEAVED, int LPR, int SIDE>
 __global__ void __launch_bounds__(AP_WARPS * 32, SIDE == 4 ? 8 : 5) paged_append_vec_kernel(PagedAppendArgs a, int parts, int* status) {

@@ -3,8 +3,8 @@
 //   s_j = f(scale q . K_j),  f(x) = x  or  softcap tanh(x / softcap)
 //   out = sum_j exp(s_j - m) V_j / sum_j exp(s_j - m),  j in [max(0, kv_len - window), kv_len),  m = max s_j
 //
-// A token that sees no position gets zeros.  Every visible key and value is read once per (token, kv head): the cache's
-// bytes are the bound (4 D bytes for 4 D H / Hkv operations), so the kernel is built around keeping loads in flight.
+// A token that sees no position gets zeros.  Every visible key and value is read once per (token, kv head, 16 of its query heads): the
+// cache's bytes are the bound (4 D bytes for 4 D H / Hkv operations), so the kernel is built around keeping loads in flight.
 //
 // Work: a (token, kv head, up to 8 or 16 of its query heads) is an item, its visible positions are cut into units of 64
 // keys.  The units of all items, in order, are dealt to a fixed grid in equal contiguous shares, from the lengths on the
@@ -14,14 +14,14 @@
 //
 // Inside a CTA each of four warps owns 16 keys of a unit and its own ring of stages, without block barriers between
 // units; the ring runs on across items.  Rows are copied by cp.async with their 16-byte pieces on neighbouring lanes: 131072 keys
-// (32 heads on 8, D = 128) take 94 us, 6.9 TB/s from one length to the next.  The same rows in 64-byte steps on four lanes
+// (32 heads on 8, D = 128) take 94 to 97 us, 5.5 to 5.7 TB/s.  When they took 94, the same rows in 64-byte steps on four lanes
 // took 122 us, as one bulk copy each 124 us (the copy engine takes one every 8 cycles, and a tile is 32 of them); keys and
 // values as two groups, refilled one after the other, 118 us; a window of 32 block-table entries in registers 100 us.
 // The products are m16n8k16 with the cache as the 16 rows and eight query heads as the columns: S^T = K Q^T (16 keys),
 // O^T += V^T P^T (16 of D).  Decode has 1 to 16 query heads a kv head, a corner of a 128-row tcgen05 tile; here the tensor
 // time is a fraction of the load time.  Weights enter the second product as two values of the cache's type, what fits the
 // first and what that left, 16 bits together in bf16 and 22 in fp16: the result's own rounding is then the only one of its size
-// (131072 keys take 96.6 us, 95.8 with weights rounded once; 64 sequences of 1 to 8192 keys in fp16 141 and 137).
+// (131072 keys take 96.9 us, 96.0 with weights rounded once; 64 sequences of 1 to 8192 keys in fp16 141 and 139).
 // Rows that are not visible are not copied: a tile that has some masks their scores, and their values too, which may be left-over NaN.
 // Maximum, sum and output are kept in 32 bits.
 #include <cuda_bf16.h>

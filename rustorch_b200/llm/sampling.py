@@ -114,7 +114,8 @@ class Sampler:
 
     def draw(self, logits: torch.Tensor, uniform: torch.Tensor) -> torch.Tensor:
         """``logits [B, V]`` and numbers ``uniform [B]`` in ``[0, 1)`` -> tokens ``[B]`` by the same settings: one kernel on CUDA
-        (``ops.sampling.sample_tokens``), a function of its arguments and the history alone."""
+        (``ops.sampling.sample_tokens``), a function of its arguments and the history alone.  Of tokens that tie at ``top_k`` it keeps
+        the first (``__call__`` keeps them all); a row without a possible token gives -1."""
         from ..ops.sampling import sample_tokens
         c = self.config
         if self.history is not None and c.repetition_penalty != 1.0:
