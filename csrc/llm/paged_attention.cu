@@ -318,8 +318,8 @@ paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, bool 
   for (int i = 0; i < S; ++i) issue(i);
 
   // ---- items
-  const float scale2 = a.softcap > 0.f ? a.scale / a.softcap : a.scale * PA_LOG2E;
-  const float cap2 = a.softcap * PA_LOG2E;
+  const float scale2 = a.softcap > 0.f ? a.scale : a.scale * PA_LOG2E;
+  const float cap2 = a.softcap * PA_LOG2E, inv_cap = 1.f / a.softcap;  // scale / softcap itself may lie below the 32-bit numbers
   float* acc_buf = reinterpret_cast<float*>(smem + C::OFF_ACC);
   float* sm_m = reinterpret_cast<float*>(smem + C::OFF_ML);
   float* sm_l = sm_m + PA_WARPS * HEADS;
@@ -392,7 +392,7 @@ paged_attention_kernel(PagedAttnArgs a, unsigned page_mul, int page_shift, bool 
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float x = (s[h][0][e] + s[h][1][e]) * scale2;
-            if (a.softcap > 0.f) x = cap2 * tanh_of(x);
+            if (a.softcap > 0.f) x = cap2 * tanh_of(x * inv_cap);
             if (!all && !(mask >> ((lane >> 2) + (e < 2 ? 0 : 8)) & 1)) x = -CUDART_INF_F;
             grow |= x > m[h][e & 1] + PA_SLACK;
             s[h][0][e] = x;

@@ -146,3 +146,22 @@ def test_infinite_values_stay_infinite(dtype, scale, heads, D):
         want = ("finite", "inf", "-inf", "nan")[d % 4] if d % 8 != 5 else "nan"
         got = out[:, d]
         assert bool({"finite": torch.isfinite(got), "inf": got == float("inf"), "-inf": got == -float("inf"), "nan": torch.isnan(got)}[want].all()), (d, want)
+
+
+@pytest.mark.parametrize("power,softcap", [(24, 1e30), (24, 0.0), (24, 2.0), (0, 1e-6), (0, 1e30)])
+def test_large_keys_small_scale_and_a_far_cap(power, softcap):
+    """Keys and queries of 2^power, a scale of 2^(-2 power): scores are small whole numbers whatever the cap's distance, although scale /
+    cap alone is below the 32-bit numbers."""
+    from rustorch_b200.ops.paged import paged_attention
+    n, D = 200, 64
+    s = torch.arange(n) % 4
+    keys, values = torch.zeros(n, D), torch.zeros(n, D)
+    keys[:, 0], values[torch.arange(n), s] = s * 2.0 ** power, 1.0
+    q = torch.zeros(1, 3, D, dtype=torch.bfloat16, device="cuda")
+    q[:, :, 0] = 2.0 ** power
+    score = s.double() if softcap == 0 or softcap == 1e30 else softcap * torch.tanh(s.double() / softcap)
+    want = torch.zeros(D, dtype=torch.float64).index_add_(0, s, torch.softmax(score, 0))
+    out = paged_attention(q, *_pages(keys, values, 16, torch.bfloat16), _i32([n]), scale=2.0 ** (-2 * power), softcap=softcap)
+    # the result's rounding; two parts of a weight (2^-16 of it); scores below 4 in eight 32-bit roundings and a tanh to 2^-21 of the cap
+    tol = want * (half_step(torch.bfloat16) + 2 * 2.0 ** -16 + 2 * 4 * (8 * 2.0 ** -24 + 2.0 ** -21)) + 2.0 ** -30
+    assert bool(((out.double().cpu() - want).abs() <= tol).all())
